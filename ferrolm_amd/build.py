@@ -24,7 +24,8 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 OBJ = PKG / "_build"
 LIB = PKG / "libferro_gpu.so"
-SOURCES = ["kernels.hip", "gemm.hip", "gemm_bf16.hip", "gemm_int8.hip", "gemm_int4.hip", "sampling.hip", "quant.hip", "api.hip"]
+SOURCES = ["kernels.hip", "gemm.hip", "gemm_bf16.hip", "gemm_int8.hip", "gemm_int4.hip", "sampling.hip", "quant.hip", "cache.hip",
+           "tree.hip", "verify.hip", "api.hip"]
 # MFMA results in VGPRs: where a workgroup fills a CU's LDS a wave may take 512 registers, and the
 # compiler would put every product into the accumulation registers and copy it out again for the VALU
 MFMA_IN_VGPRS = ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]

@@ -5,6 +5,7 @@
 #include "ferro_gpu.h"
 #include "ferro_host.h"
 #include "internal.h"
+#include "rows.h"
 
 #include <algorithm>
 #include <atomic>
@@ -130,6 +131,7 @@ struct fg_ctx {
     size_t hmeta_cap = 0;
     Stage stage;  // slots for large host copies of load-time calls
     hipEvent_t ev[3] = {nullptr, nullptr, nullptr};
+    hipEvent_t order[2] = {nullptr, nullptr};  // fg_ctx_wait_stream, fg_stream_wait_ctx
     float last_us[3] = {0, 0, 0};
     bool merge_in_o = true;  // small bf16 output projections merge the attention spans themselves
     bool mlp_fuse = true;    // bf16 layers of one pass run fused (mlp_fuse: split output projection, EPI_MLP)
@@ -279,15 +281,71 @@ struct fg_model {
 struct fg_kv {
     uint64_t serial = g_serial++;
     int layers = 0, kv_heads = 0, head_dim = 0, block_size = 0, blocks = 0;
+    int format = KV_F32;
     float* k = nullptr;  // [layer][blocks*bs*nkv*hd]
     float* v = nullptr;
+    uint8_t* data = nullptr;  // 8-bit formats: [layer][block][kv head][record]
     size_t layer_floats() const { return (size_t)blocks * block_size * kv_heads * head_dim; }
+    size_t layer_bytes() const {
+        return format == KV_F32 ? layer_floats() * 4 : (size_t)blocks * kv_heads * kv_record(head_dim);
+    }
+    KvLayer layer(int i) const {
+        KvLayer l;
+        l.format = format;
+        l.nkv = kv_heads;
+        l.hd = head_dim;
+        if (format == KV_F32) {
+            l.k = k + i * layer_floats();
+            l.v = v + i * layer_floats();
+        } else {
+            l.data = data + i * layer_bytes();
+        }
+        return l;
+    }
 };
 
 struct fg_mat {
     DMat m;
     int device = 0;
 };
+
+// Rows over a cache (fg_rows_create): the plan, its device copy, and the attention's partials.
+struct fg_rows {
+    fg_ctx* ctx = nullptr;
+    int device = 0;
+    int heads = 1, kv_heads = 1, head_dim = 64, kv_blocks = 0;  // kv_blocks 0: no cache
+    RowPlan plan;
+    bool ready = false;
+    void *hmeta = nullptr, *dmeta = nullptr, *part = nullptr;
+    size_t hmeta_cap = 0, dmeta_cap = 0, part_cap = 0;
+    hipEvent_t sent = nullptr;  // the plan's copy to the device
+    RowArgs args() const { return row_args(plan, (const int32_t*)dmeta); }
+};
+
+// The current device for a call, put back after it.
+struct DeviceScope {
+    int before = -1;
+    explicit DeviceScope(int device) {
+        if (hipGetDevice(&before) != hipSuccess || before == device)
+            before = -1;
+        else
+            (void)hipSetDevice(device);
+    }
+    DeviceScope(const DeviceScope&) = delete;
+    ~DeviceScope() {
+        if (before >= 0) (void)hipSetDevice(before);
+    }
+};
+
+// f()'s code; a C++ exception (out of host memory) becomes an error code.
+template <class F>
+static int guarded(const F& f) {
+    try {
+        return f();
+    } catch (const std::exception& e) {
+        return fail(FG_E_NOMEM, e.what());
+    }
+}
 
 static int ensure(void** p, size_t* cap, size_t need, hipStream_t st, bool host) {
     if (need <= *cap && *p) return 0;
@@ -473,6 +531,8 @@ struct ChunkIn {
     int n, pos;
     const uint32_t* blocks;
     int n_blocks, logits;
+    const int32_t* parents = nullptr;  // a tree's; nullptr: a chain
+    bool tree = false;                 // fg_forward_tree: planned as rows, whatever the cache
 };
 
 struct Plan {
@@ -492,6 +552,10 @@ struct Plan {
     // item, W counts two partial slots per item); btab holds the block tables
     // of the chunks the items read
     bool flash = false;
+    // rows: 8-bit caches and trees, whose attention takes the plan in `rp` (packed at o_rows) instead
+    bool rows = false;
+    RowPlan rp;
+    size_t o_rows = 0;
     std::vector<int32_t> btab;
     // offsets (in int32 words) of each array inside the packed metadata
     size_t o_wrec, o_mrec, o_sel, o_tok, o_btab, words;
@@ -512,6 +576,9 @@ static int build_plan(const fg_config& c, const fg_kv& kv, int max_pos, const Ch
     const int span1 = attn_span(c.head_dim);
     if (bs != 16 || span1 % bs || span1 / bs > 8) return fail(FG_E_SHAPE, "attention spans need 16-token blocks");
     P = Plan();
+    P.rows = kv.format != KV_F32;
+    for (int ci = 0; ci < nch; ci++) P.rows = P.rows || ch[ci].tree;
+    std::vector<RowSeq> rseq;
     // Work items of one span, or, when they would be more than 1024 workgroups
     // and a row group reaches kAttnMfmaQueries queries (GQA verify batches,
     // prefill chunks), of 128 positions: 2 or 4 sub-spans whose loads overlap
@@ -583,7 +650,7 @@ static int build_plan(const fg_config& c, const fg_kv& kv, int max_pos, const Ch
             fpart /= 2;
             parts = count();
         }
-        P.flash = parts >= (fill && c.head_dim == 64 ? 96 : 256);
+        P.flash = !P.rows && parts >= (fill && c.head_dim == 64 ? 96 : 256);
         if (P.flash) P.ns = 1;
     }
     for (int ci = 0; ci < nch; ci++) {
@@ -606,7 +673,9 @@ static int build_plan(const fg_config& c, const fg_kv& kv, int max_pos, const Ch
                 P.tokens.push_back(0);
             }
         }
-        if (P.flash) {
+        if (P.rows) {
+            rseq.push_back(RowSeq{k.n, k.pos, k.blocks, k.n_blocks, k.parents});
+        } else if (P.flash) {
             const int boff = (int)P.btab.size();
             for (int b = 0; b < used; b++) P.btab.push_back((int32_t)k.blocks[b]);
             for (int r0 = 0; r0 < k.n; r0 += rf) {
@@ -661,9 +730,13 @@ static int build_plan(const fg_config& c, const fg_kv& kv, int max_pos, const Ch
     // captures the step's graphs again: cfg3 at 32 sequences, 48 steps,
     // 2627-2649 -> 2716-2723 tok/s with this rounding)
     int wstep = 16;
+    if (P.rows) {
+        plan_rows(P.rp, rseq.data(), (int)rseq.size(), c.heads, c.kv_heads, c.head_dim, true);
+        P.W = P.rp.n_wi;
+    }
     while (wstep * 16 <= P.W) wstep *= 2;
     P.Wc = std::max(16, (P.W + wstep - 1) / wstep * wstep);
-    P.wrec.resize((size_t)P.Wc * 16, 0);
+    P.wrec.resize(P.rows ? 0 : (size_t)P.Wc * 16, 0);
     size_t o = 0;
     auto place = [&](size_t n) {
         size_t r = o;
@@ -675,6 +748,7 @@ static int build_plan(const fg_config& c, const fg_kv& kv, int max_pos, const Ch
     P.o_sel = place(P.S);
     P.o_tok = place(P.t);
     P.o_btab = place(P.btab.size());
+    P.o_rows = place(P.rp.words);
     P.words = o;
     return 0;
 }
@@ -688,6 +762,7 @@ static void pack_plan(const Plan& P, int32_t* h) {
     cp(P.o_sel, P.sel);
     if (!P.tokens.empty()) memcpy(h + P.o_tok, P.tokens.data(), P.tokens.size() * 4);
     cp(P.o_btab, P.btab);
+    if (P.rows) pack_rows(P.rp, h + P.o_rows);
 }
 
 // Workspace of one forward pass over a plan.
@@ -904,6 +979,11 @@ static int run_forward(fg_ctx* ctx, const fg_model* m, fg_kv* kv, const Plan& P,
     aa.hd = hd;
     aa.bs = kv->block_size;
     aa.scale = 1.0f / sqrtf((float)hd);
+    RowArgs ra;
+    if (P.rows) {
+        ra = row_args(P.rp, meta + P.o_rows);
+        aa.mrec = ra.mrec;
+    }
 
     // When every row's logits are selected, in order (draft rounds, verify
     // steps), the last layer's down projection writes the lm_head's pieces of
@@ -958,13 +1038,31 @@ static int run_forward(fg_ctx* ctx, const fg_model* m, fg_kv* kv, const Plan& P,
         }
         gemv(ctx, EPI_QKV, l.wqkv, g);
         // attention (RoPE, cache write) and the merge into wo's pieces
-        aa.kc = kv->k + li * kv->layer_floats();
-        aa.vc = kv->v + li * kv->layer_floats();
+        if (!P.rows) {
+            aa.kc = kv->k + li * kv->layer_floats();
+            aa.vc = kv->v + li * kv->layer_floats();
+        }
         Pieces po = pieces(w, cur ^ 1, l.wo.kb, passes);
         const bool am = fuse_l || (ctx->merge_in_o && merge_in_o(c, P, l.wo, mm));
         aa.stamp = next_stamp(ctx, "attention");
         if (!am && aa.stamp >= 0) next_stamp(ctx, "merge");  // the merge launch takes the next slot
-        if (launch_attention(st, aa, t, am ? -1 : ck(l.wo), po))
+        if (P.rows) {
+            // the new keys and values into the cache (rotated, quantized), then the rows over it; the
+            // partials and their merge are the other kernels'
+            const KvLayer kl = kv->layer(li);
+            TreeAttn ta;
+            ta.q = w.qkv;
+            ta.ldq = aa.ld;
+            ta.part = w.apart;
+            ta.nh = nh;
+            ta.scale = aa.scale;
+            ta.cos_t = m->cos_t;
+            ta.sin_t = m->sin_t;
+            const float* kp = w.qkv + (size_t)nh * hd;
+            if (launch_kv_append(st, ra, kl, kp, kp + (size_t)nkv * hd, aa.ld, m->cos_t, m->sin_t) ||
+                launch_tree_attn(st, ra, kl, ta) || launch_merge(st, aa, t, am ? -1 : ck(l.wo), po))
+                return fail(FG_E_SHAPE, "no attention kernel for head_dim " + std::to_string(hd));
+        } else if (launch_attention(st, aa, t, am ? -1 : ck(l.wo), po))
             return fail(FG_E_SHAPE, "no attention kernel for head_dim " + std::to_string(hd));
         if (cap && launch_cap_merge(st, aa, t, capl + (size_t)t * H, qd))
             return fail(FG_E_SHAPE, "no attention kernel for head_dim " + std::to_string(hd));
@@ -1331,6 +1429,8 @@ void fg_ctx_destroy(fg_ctx* c) {
     if (c->gcnt) (void)hipFree(c->gcnt);
     for (auto& e : c->ev)
         if (e) (void)hipEventDestroy(e);
+    for (auto& e : c->order)
+        if (e) (void)hipEventDestroy(e);
     for (auto& e : c->pev) (void)hipEventDestroy(e);
     (void)hipStreamDestroy(c->stream);
     delete c;
@@ -1443,8 +1543,14 @@ int64_t fg_model_weight_bytes(const fg_model* m) { return m ? m->ref_bytes : 0; 
 
 int fg_kv_create(fg_ctx* ctx, int32_t layers, int32_t kv_heads, int32_t head_dim, int32_t block_size, int32_t blocks,
                  fg_kv** out) {
+    return fg_kv_create_format(ctx, layers, kv_heads, head_dim, block_size, blocks, FG_KV_F32, out);
+}
+
+int fg_kv_create_format(fg_ctx* ctx, int32_t layers, int32_t kv_heads, int32_t head_dim, int32_t block_size,
+                        int32_t blocks, int32_t format, fg_kv** out) {
     if (!ctx || !out || layers <= 0 || kv_heads <= 0 || head_dim <= 0 || block_size != 16 || blocks <= 0)
         return fail(FG_E_ARG, "bad cache shape (block_size must be 16)");
+    if (format < FG_KV_F32 || format > FG_KV_FP8) return fail(FG_E_ARG, "unknown cache format");
     if (!head_dim_supported(head_dim))
         return fail(FG_E_SHAPE, "head_dim " + std::to_string(head_dim) +
                                     " has no device attention kernel (supported: 16, 32, 64, 128)");
@@ -1455,16 +1561,21 @@ int fg_kv_create(fg_ctx* ctx, int32_t layers, int32_t kv_heads, int32_t head_dim
     kv->head_dim = head_dim;
     kv->block_size = block_size;
     kv->blocks = blocks;
-    const size_t bytes = kv->layer_floats() * layers * 4;
-    if (hipMalloc((void**)&kv->k, bytes) != hipSuccess || hipMalloc((void**)&kv->v, bytes) != hipSuccess) {
+    kv->format = format;
+    const size_t bytes = kv->layer_bytes() * layers;
+    const bool ok = format == FG_KV_F32
+                        ? hipMalloc((void**)&kv->k, bytes) == hipSuccess && hipMalloc((void**)&kv->v, bytes) == hipSuccess
+                        : hipMalloc((void**)&kv->data, bytes) == hipSuccess;
+    if (!ok) {
         fg_kv_destroy(kv);
         return fail(FG_E_NOMEM, "cache allocation failed");
     }
     // clear before the handle is returned: contexts' streams do not wait for each other or for the
     // default stream, and any context on the device may write the cache's first rows
-    if (hipMemsetAsync(kv->k, 0, bytes, ctx->stream) != hipSuccess ||
-        hipMemsetAsync(kv->v, 0, bytes, ctx->stream) != hipSuccess ||
-        hipStreamSynchronize(ctx->stream) != hipSuccess) {
+    bool clear = true;
+    for (void* p : {(void*)kv->k, (void*)kv->v, (void*)kv->data})
+        clear = clear && (!p || hipMemsetAsync(p, 0, bytes, ctx->stream) == hipSuccess);
+    if (!clear || hipStreamSynchronize(ctx->stream) != hipSuccess) {
         fg_kv_destroy(kv);
         return fail(FG_E_DEVICE, "cache clear failed");
     }
@@ -1476,14 +1587,25 @@ void fg_kv_destroy(fg_kv* kv) {
     if (!kv) return;
     if (kv->k) (void)hipFree(kv->k);
     if (kv->v) (void)hipFree(kv->v);
+    if (kv->data) (void)hipFree(kv->data);
     delete kv;
 }
 
 int fg_kv_read(fg_ctx* ctx, const fg_kv* kv, int32_t layer, float* k_out, float* v_out) {
     if (!ctx || !kv || layer < 0 || layer >= kv->layers || !k_out || !v_out) return fail(FG_E_ARG, "bad argument");
     const size_t n = kv->layer_floats();
-    HIPCHK(hipMemcpyAsync(k_out, kv->k + layer * n, n * 4, hipMemcpyDeviceToHost, ctx->stream));
-    HIPCHK(hipMemcpyAsync(v_out, kv->v + layer * n, n * 4, hipMemcpyDeviceToHost, ctx->stream));
+    const float *k = kv->k + layer * n, *v = kv->v + layer * n;
+    DevBuf buf;
+    if (kv->format != KV_F32) {
+        HIPCHK(hipSetDevice(ctx->device));
+        if (int rc = dev_alloc(buf, n * 8)) return rc;
+        k = (const float*)buf.p;
+        v = k + n;
+        launch_kv_unpack(ctx->stream, kv->layer(layer), kv->blocks, (float*)k, (float*)v);
+        HIPCHK(hipGetLastError());
+    }
+    HIPCHK(hipMemcpyAsync(k_out, k, n * 4, hipMemcpyDeviceToHost, ctx->stream));
+    HIPCHK(hipMemcpyAsync(v_out, v, n * 4, hipMemcpyDeviceToHost, ctx->stream));
     HIPCHK(hipStreamSynchronize(ctx->stream));
     return 0;
 }
@@ -1491,8 +1613,20 @@ int fg_kv_read(fg_ctx* ctx, const fg_kv* kv, int32_t layer, float* k_out, float*
 int fg_kv_write(fg_ctx* ctx, fg_kv* kv, int32_t layer, const float* k, const float* v) {
     if (!ctx || !kv || layer < 0 || layer >= kv->layers || !k || !v) return fail(FG_E_ARG, "bad argument");
     const size_t n = kv->layer_floats();
-    HIPCHK(hipMemcpyAsync(kv->k + layer * n, k, n * 4, hipMemcpyHostToDevice, ctx->stream));
-    HIPCHK(hipMemcpyAsync(kv->v + layer * n, v, n * 4, hipMemcpyHostToDevice, ctx->stream));
+    float *dk = kv->k + layer * n, *dv = kv->v + layer * n;
+    DevBuf buf;
+    if (kv->format != KV_F32) {
+        HIPCHK(hipSetDevice(ctx->device));
+        if (int rc = dev_alloc(buf, n * 8)) return rc;
+        dk = (float*)buf.p;
+        dv = dk + n;
+    }
+    HIPCHK(hipMemcpyAsync(dk, k, n * 4, hipMemcpyHostToDevice, ctx->stream));
+    HIPCHK(hipMemcpyAsync(dv, v, n * 4, hipMemcpyHostToDevice, ctx->stream));
+    if (kv->format != KV_F32) {
+        launch_kv_pack(ctx->stream, kv->layer(layer), kv->blocks, dk, dv);
+        HIPCHK(hipGetLastError());
+    }
     HIPCHK(hipStreamSynchronize(ctx->stream));
     return 0;
 }
@@ -1781,6 +1915,12 @@ static int spec_step(fg_ctx* ctx, const fg_model* target, fg_kv* tkv, const fg_m
             for (int64_t v : {(int64_t)P.t, (int64_t)P.S, (int64_t)P.Wc, (int64_t)P.words, (int64_t)P.ns,
                               (int64_t)P.flash, (int64_t)P.maxq})
                 sig.push_back(v);
+            if (P.rows)
+                for (int64_t v : {(int64_t)P.rp.n_items, (int64_t)P.rp.n_quads, (int64_t)P.rp.qt, (int64_t)P.rp.rw,
+                                  (int64_t)P.rp.pw, (int64_t)P.rp.o_items, (int64_t)P.rp.o_mrec, (int64_t)P.rp.o_quads,
+                                  (int64_t)P.rp.o_rpos, (int64_t)P.rp.o_masks, (int64_t)P.o_sel, (int64_t)P.o_tok,
+                                  (int64_t)P.o_rows})
+                    sig.push_back(v);
         }
         for (auto& g : ctx->gsets)
             if (g.sig == sig) gset = &g;
@@ -2308,6 +2448,398 @@ int fg_awq_search(fg_ctx* ctx, int32_t kind, int32_t rows, int32_t k, const floa
     choice->error_plain = plain;
     choice->error_awq = best;
     return 0;
+}
+
+// ---- rows over paged caches ------------------------------------------------
+
+int fg_ctx_wait_stream(fg_ctx* ctx, void* stream) {
+    if (!ctx) return fail(FG_E_ARG, "null ctx");
+    const DeviceScope on(ctx->device);
+    if (!ctx->order[0]) HIPCHK(hipEventCreateWithFlags(&ctx->order[0], hipEventDisableTiming));
+    HIPCHK(hipEventRecord(ctx->order[0], (hipStream_t)stream));
+    HIPCHK(hipStreamWaitEvent(ctx->stream, ctx->order[0], 0));
+    return 0;
+}
+
+int fg_stream_wait_ctx(fg_ctx* ctx, void* stream) {
+    if (!ctx) return fail(FG_E_ARG, "null ctx");
+    const DeviceScope on(ctx->device);
+    if (!ctx->order[1]) HIPCHK(hipEventCreateWithFlags(&ctx->order[1], hipEventDisableTiming));
+    HIPCHK(hipEventRecord(ctx->order[1], ctx->stream));
+    HIPCHK(hipStreamWaitEvent((hipStream_t)stream, ctx->order[1], 0));
+    return 0;
+}
+
+// parents of n rows: -1, an earlier row in use, or -2 (an unused row; where it may be).
+static int check_parents(const int32_t* parents, int32_t n, bool unused) {
+    bool chain = true;
+    for (int i = 0; parents && i < n; i++) {
+        if (parents[i] < -2 || parents[i] >= i) return fail(FG_E_ARG, "a row's parent must be an earlier row, -1 or -2");
+        if (parents[i] == -2 && !unused) return fail(FG_E_ARG, "unused rows are not taken here");
+        if (parents[i] >= 0 && parents[parents[i]] == -2) return fail(FG_E_ARG, "an unused row has no children");
+        chain = chain && parents[i] == i - 1;
+    }
+    if (!chain && n > kTreeRows) return fail(FG_E_SHAPE, "a tree has at most " + std::to_string(kTreeRows) + " rows");
+    return 0;
+}
+
+static int rows_plan(fg_rows* r, const fg_tree_seq* seqs, int32_t n_seqs) {
+    if (n_seqs < 0 || (n_seqs > 0 && !seqs)) return fail(FG_E_ARG, "null sequences");
+    if (n_seqs > 65535) return fail(FG_E_SHAPE, "at most 65535 sequences");
+    const bool cached = r->kv_blocks > 0;
+    std::vector<RowSeq> in(n_seqs);
+    int64_t rows = 0, tokens = 0;
+    for (int s = 0; s < n_seqs; s++) {
+        const fg_tree_seq& q = seqs[s];
+        if (q.n < 0 || q.pos < 0) return fail(FG_E_ARG, "negative row count or position");
+        const int64_t last = (int64_t)q.pos + q.n;
+        if (last > (1 << 30)) return fail(FG_E_SHAPE, "position beyond 2^30");
+        if (int rc = check_parents(q.parents, q.n, true)) return rc;
+        if (cached) {
+            if (last > 0 && !q.blocks) return fail(FG_E_ARG, "sequence without a block table");
+            if ((int64_t)q.n_blocks * 16 < last) return fail(FG_E_SHAPE, "rows overrun their cache blocks");
+            for (int64_t b = 0; b * 16 < last; b++)
+                if (q.blocks[b] >= (uint32_t)r->kv_blocks) return fail(FG_E_ARG, "block id beyond the cache");
+        }
+        rows += q.n;
+        tokens += last;
+        in[s] = RowSeq{q.n, q.pos, q.blocks, q.n_blocks, q.parents};
+    }
+    if (rows > (1 << 24) || tokens > INT32_MAX) return fail(FG_E_SHAPE, "too many rows or tokens");
+    plan_rows(r->plan, in.data(), n_seqs, r->heads, r->kv_heads, r->head_dim, cached);
+    const RowPlan& P = r->plan;
+    // the staging may still be on its way up for the plan before
+    if (r->sent) HIPCHK(hipEventSynchronize(r->sent));
+    int rc;
+    if ((rc = ensure(&r->hmeta, &r->hmeta_cap, P.words * 4, r->ctx->stream, true)) ||
+        (rc = ensure(&r->dmeta, &r->dmeta_cap, P.words * 4, r->ctx->stream, false)))
+        return rc;
+    if (P.parts && (rc = ensure(&r->part, &r->part_cap,
+                                (size_t)P.n_wi * r->kv_heads * attn_qmax(r->head_dim) * (r->head_dim + 4) * 4,
+                                r->ctx->stream, false)))
+        return rc;
+    if (!r->sent) HIPCHK(hipEventCreateWithFlags(&r->sent, hipEventDisableTiming));
+    pack_rows(P, (int32_t*)r->hmeta);
+    HIPCHK(hipMemcpyAsync(r->dmeta, r->hmeta, P.words * 4, hipMemcpyHostToDevice, r->ctx->stream));
+    HIPCHK(hipEventRecord(r->sent, r->ctx->stream));
+    r->ready = true;
+    return 0;
+}
+
+int fg_rows_create(fg_ctx* ctx, const fg_kv* kv, int32_t heads, const fg_tree_seq* seqs, int32_t n_seqs,
+                   fg_rows** out) {
+    if (!ctx || !out) return fail(FG_E_ARG, "null argument");
+    if (kv) {
+        if (heads <= 0 || heads % kv->kv_heads) return fail(FG_E_SHAPE, "query heads must be a multiple of the kv heads");
+        if (heads / kv->kv_heads > attn_qmax(kv->head_dim)) return fail(FG_E_SHAPE, "GQA group too large");
+    }
+    const DeviceScope on(ctx->device);
+    fg_rows* r = new fg_rows();
+    r->ctx = ctx;
+    r->device = ctx->device;
+    if (kv) {
+        r->heads = heads;
+        r->kv_heads = kv->kv_heads;
+        r->head_dim = kv->head_dim;
+        r->kv_blocks = kv->blocks;
+    }
+    const int rc = guarded([&] { return rows_plan(r, seqs, n_seqs); });
+    if (rc) {
+        const std::string why = g_err;
+        fg_rows_destroy(r);
+        g_err = why;
+        return rc;
+    }
+    *out = r;
+    return 0;
+}
+
+int fg_rows_set(fg_rows* r, const fg_tree_seq* seqs, int32_t n_seqs) {
+    if (!r) return fail(FG_E_ARG, "null rows");
+    const DeviceScope on(r->ctx->device);
+    hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+    HIPCHK(hipStreamIsCapturing(r->ctx->stream, &cap));
+    if (cap != hipStreamCaptureStatusNone) return fail(FG_E_ARG, "rows can't be planned while the context's stream is captured");
+    r->ready = false;
+    return guarded([&] { return rows_plan(r, seqs, n_seqs); });
+}
+
+void fg_rows_destroy(fg_rows* r) {
+    if (!r) return;
+    const DeviceScope on(r->device);  // the context may be gone already
+    if (r->dmeta) (void)hipFree(r->dmeta);  // waits for queued work that uses it
+    if (r->part) (void)hipFree(r->part);
+    if (r->hmeta) (void)hipHostFree(r->hmeta);
+    if (r->sent) (void)hipEventDestroy(r->sent);
+    delete r;
+}
+
+int fg_rows_count(const fg_rows* r, int32_t* rows, int64_t* tokens, int32_t* deepest) {
+    if (!r || !r->ready) return fail(FG_E_ARG, "rows without a plan");
+    if (rows) *rows = r->plan.rows;
+    if (tokens) *tokens = r->plan.tokens;
+    if (deepest) *deepest = r->plan.deepest;
+    return 0;
+}
+
+// The context, the rows and (kv) one layer of a cache fit each other.
+static int check_rows(const fg_ctx* ctx, const fg_rows* r, const fg_kv* kv, int32_t layer) {
+    if (!ctx || !r || !kv) return fail(FG_E_ARG, "null argument");
+    if (r->ctx != ctx || !r->ready) return fail(FG_E_ARG, "the rows are another context's, or without a plan");
+    if (layer < 0 || layer >= kv->layers) return fail(FG_E_ARG, "no such layer");
+    if (!r->kv_blocks || r->kv_heads != kv->kv_heads || r->head_dim != kv->head_dim)
+        return fail(FG_E_SHAPE, "the rows were planned for another cache shape");
+    if (!r->plan.btab.empty() && r->plan.top_block >= (uint32_t)kv->blocks) return fail(FG_E_ARG, "block id beyond the cache");
+    return 0;
+}
+static int check_array(const void* p, int64_t ld, int64_t width) {
+    if (!p) return fail(FG_E_ARG, "null array");
+    if (ld < width || ld % 4 || (uintptr_t)p % 16)
+        return fail(FG_E_SHAPE, "rows must be 16-byte aligned and at least as far apart as they are wide");
+    return 0;
+}
+
+int fg_kv_append(fg_ctx* ctx, const fg_rows* r, fg_kv* kv, int32_t layer, const float* k_dev, const float* v_dev,
+                 int64_t ld) {
+    int rc;
+    if ((rc = check_rows(ctx, r, kv, layer))) return rc;
+    if (r->plan.rows == 0) return 0;
+    const int64_t width = (int64_t)kv->kv_heads * kv->head_dim;
+    if ((rc = check_array(k_dev, ld, width)) || (rc = check_array(v_dev, ld, width))) return rc;
+    const DeviceScope on(ctx->device);
+    launch_kv_append(ctx->stream, r->args(), kv->layer(layer), k_dev, v_dev, ld, nullptr, nullptr);
+    HIPCHK(hipGetLastError());
+    return 0;
+}
+
+int fg_kv_gather(fg_ctx* ctx, const fg_rows* r, const fg_kv* kv, int32_t layer, int32_t context, float* k_dev,
+                 float* v_dev) {
+    int rc;
+    if ((rc = check_rows(ctx, r, kv, layer))) return rc;
+    if ((context ? r->plan.tokens : r->plan.rows) == 0) return 0;
+    const int64_t width = (int64_t)kv->kv_heads * kv->head_dim;
+    if ((rc = check_array(k_dev, width, width)) || (rc = check_array(v_dev, width, width))) return rc;
+    const DeviceScope on(ctx->device);
+    launch_kv_gather(ctx->stream, r->args(), kv->layer(layer), context != 0, k_dev, v_dev);
+    HIPCHK(hipGetLastError());
+    return 0;
+}
+
+int fg_kv_commit(fg_ctx* ctx, const fg_rows* r, fg_kv* kv, const int32_t* path_dev, const int32_t* count_dev,
+                 int32_t ld) {
+    int rc;
+    if ((rc = check_rows(ctx, r, kv, 0))) return rc;
+    if (r->plan.rows == 0) return 0;
+    if (!path_dev || !count_dev || ld < 0) return fail(FG_E_ARG, "bad argument");
+    const DeviceScope on(ctx->device);
+    launch_kv_commit(ctx->stream, r->args(), kv->layer(0), kv->layers, kv->layer_bytes(), path_dev, count_dev, ld);
+    HIPCHK(hipGetLastError());
+    return 0;
+}
+
+int fg_tree_attention(fg_ctx* ctx, const fg_rows* r, const fg_kv* kv, int32_t layer, const float* q_dev, int64_t ldq,
+                      float* out_dev, int64_t ldo) {
+    int rc;
+    if ((rc = check_rows(ctx, r, kv, layer))) return rc;
+    if (r->plan.rows == 0) return 0;
+    const int64_t width = (int64_t)r->heads * r->head_dim;
+    if ((rc = check_array(q_dev, ldq, width)) || (rc = check_array(out_dev, ldo, width))) return rc;
+    const DeviceScope on(ctx->device);
+    TreeAttn t;
+    t.q = q_dev;
+    t.ldq = ldq;
+    t.out = out_dev;
+    t.ldo = ldo;
+    t.part = (float*)r->part;
+    t.nh = r->heads;
+    t.scale = 1.0f / sqrtf((float)r->head_dim);
+    launch_tree_attn(ctx->stream, r->args(), kv->layer(layer), t);
+    HIPCHK(hipGetLastError());
+    return 0;
+}
+
+static int check_tree(const fg_ctx* ctx, const fg_rows* r, int32_t ld) {
+    if (!ctx || !r) return fail(FG_E_ARG, "null argument");
+    if (r->ctx != ctx || !r->ready) return fail(FG_E_ARG, "the rows are another context's, or without a plan");
+    if (!r->plan.rooted) return fail(FG_E_ARG, "every sequence's first row must be the root of its others");
+    if (ld < r->plan.deepest)
+        return fail(FG_E_SHAPE, "the outputs hold fewer tokens than the longest branch has rows (" +
+                                    std::to_string(r->plan.deepest) + ")");
+    return 0;
+}
+
+int fg_tree_verify(fg_ctx* ctx, const fg_rows* r, int32_t drafts, int32_t vocab, const uint32_t* tokens_dev,
+                   const float* p_dev, const float* q_dev, const float* u_dev, uint32_t* out_tokens_dev,
+                   int32_t* out_path_dev, int32_t* out_count_dev, int32_t ld) {
+    int rc;
+    if ((rc = check_tree(ctx, r, ld))) return rc;
+    if (drafts < FG_DRAFT_EACH || drafts > FG_DRAFT_FIXED || vocab <= 0) return fail(FG_E_ARG, "bad argument");
+    if (r->plan.rows == 0) return 0;
+    if (!tokens_dev || !p_dev || !u_dev || !out_tokens_dev || !out_path_dev || !out_count_dev ||
+        (drafts == FG_DRAFT_FIXED) != !q_dev)
+        return fail(FG_E_ARG, "null array (drafts that were drawn come with q, given ones without)");
+    const DeviceScope on(ctx->device);
+    VerifyArgs v;
+    v.tokens = tokens_dev;
+    v.p = p_dev;
+    v.q = q_dev;
+    v.u = u_dev;
+    v.vocab = vocab;
+    v.kind = drafts;
+    v.out_tokens = out_tokens_dev;
+    v.out_path = out_path_dev;
+    v.out_count = out_count_dev;
+    v.ld = ld;
+    launch_tree_verify(ctx->stream, r->args(), v);
+    HIPCHK(hipGetLastError());
+    return 0;
+}
+
+int fg_tree_accept(fg_ctx* ctx, const fg_rows* r, const uint32_t* tokens_dev, const uint32_t* argmax_dev,
+                   uint32_t* out_tokens_dev, int32_t* out_path_dev, int32_t* out_count_dev, int32_t ld) {
+    int rc;
+    if ((rc = check_tree(ctx, r, ld))) return rc;
+    if (r->plan.rows == 0) return 0;
+    if (!tokens_dev || !argmax_dev || !out_tokens_dev || !out_path_dev || !out_count_dev)
+        return fail(FG_E_ARG, "null array");
+    const DeviceScope on(ctx->device);
+    launch_tree_accept(ctx->stream, r->args(), tokens_dev, argmax_dev, out_tokens_dev, out_path_dev, out_count_dev, ld);
+    HIPCHK(hipGetLastError());
+    return 0;
+}
+
+// ---- forwards over trees ---------------------------------------------------
+
+// The trees' forward with every row's logits, queued: the plan, the workspace and the device copy of the
+// metadata, `more` words behind which the caller has filled in (fill(host words)).
+static int tree_forward(fg_ctx* ctx, const fg_model* m, fg_kv* kv, const fg_tree_seq* seqs, int32_t n_seqs, Plan& P,
+                        Work& w, size_t more, const std::function<void(int32_t*)>& fill, bool logits) {
+    if (!ctx || !m || !kv || n_seqs < 0 || (n_seqs > 0 && !seqs)) return fail(FG_E_ARG, "null argument");
+    int rc;
+    if ((rc = check_model_kv(m, kv))) return rc;
+    std::vector<ChunkIn> in(n_seqs);
+    for (int s = 0; s < n_seqs; s++) {
+        const fg_tree_seq& q = seqs[s];
+        if (q.n < 0 || q.pos < 0) return fail(FG_E_ARG, "negative row count or position");
+        if (q.n > 0 && !q.tokens) return fail(FG_E_ARG, "tree without tokens");
+        if ((rc = check_parents(q.parents, q.n, false))) return rc;
+        in[s] = ChunkIn{q.tokens, q.n, q.pos, q.blocks, q.n_blocks, FG_LOGITS_ALL, q.parents, true};
+    }
+    ctx->stamp_seq = 0;
+    if ((rc = build_plan(m->cfg, *kv, m->max_pos, in.data(), n_seqs, P))) return rc;
+    if (P.t == 0) return 0;
+    const size_t words = P.words + more;
+    if ((rc = ensure(&ctx->hmeta, &ctx->hmeta_cap, words * 4, ctx->stream, true))) return rc;
+    if ((rc = ensure(&ctx->dmeta, &ctx->dmeta_cap, words * 4, ctx->stream, false))) return rc;
+    pack_plan(P, (int32_t*)ctx->hmeta);
+    fill((int32_t*)ctx->hmeta + P.words);
+    HIPCHK(hipMemcpyAsync(ctx->dmeta, ctx->hmeta, words * 4, hipMemcpyHostToDevice, ctx->stream));
+    if ((rc = ensure(&ctx->ws, &ctx->ws_cap, layout_work(m, P, w, nullptr), ctx->stream, false))) return rc;
+    layout_work(m, P, w, ctx->ws);
+    const int32_t* meta = (const int32_t*)ctx->dmeta;
+    return run_forward(ctx, m, kv, P, meta, (const uint32_t*)(meta + P.o_tok), 1, w, logits ? w.logits : nullptr,
+                       nullptr, nullptr, 0, 0, nullptr);
+}
+
+int fg_forward_tree(fg_ctx* ctx, const fg_model* m, fg_kv* kv, const fg_tree_seq* seqs, int32_t n_seqs,
+                    float* logits_out, uint32_t* argmax_out) {
+    if (!ctx) return fail(FG_E_ARG, "null argument");
+    const DeviceScope on(ctx->device);
+    return guarded([&]() -> int {
+        Plan P;
+        Work w{};
+        if (int rc = tree_forward(ctx, m, kv, seqs, n_seqs, P, w, 0, [](int32_t*) {}, logits_out != nullptr)) return rc;
+        if (P.t == 0) return 0;
+        if (logits_out)
+            HIPCHK(hipMemcpyAsync(logits_out, w.logits, (size_t)P.S * m->cfg.vocab * 4, hipMemcpyDeviceToHost, ctx->stream));
+        if (argmax_out)
+            HIPCHK(hipMemcpyAsync(argmax_out, w.am, (size_t)P.S * 4, hipMemcpyDeviceToHost, ctx->stream));
+        HIPCHK(hipStreamSynchronize(ctx->stream));
+        return 0;
+    });
+}
+
+int fg_tree_step(fg_ctx* ctx, const fg_model* m, fg_kv* kv, const fg_tree_seq* seqs, int32_t n_seqs,
+                 const fg_sampling* params, const float* u, uint32_t* out_tokens, int32_t* out_path,
+                 int32_t* out_count, int32_t ld) {
+    if (!ctx || !m || !kv || n_seqs <= 0 || !seqs || !out_tokens || !out_path || !out_count || (params && !u) || ld <= 0)
+        return fail(FG_E_ARG, "bad argument");
+    const DeviceScope on(ctx->device);
+    return guarded([&]() -> int {
+        int rc;
+        bool wide = false, sampling = false;
+        if (params) {
+            if ((rc = check_sampling(params, n_seqs, &wide))) return rc;
+            for (int s = 0; s < n_seqs; s++) sampling |= params[s].temperature > 0.0f;
+        }
+        size_t rows = 0;
+        for (int s = 0; s < n_seqs; s++) {
+            const fg_tree_seq& q = seqs[s];
+            if (q.n <= 0) return fail(FG_E_ARG, "a tree has at least one row");
+            if ((rc = check_parents(q.parents, q.n, false))) return rc;
+            int deepest = 0;
+            std::vector<int> depth(q.n);
+            for (int i = 0; i < q.n; i++) {
+                const int p = q.parents ? q.parents[i] : i - 1;
+                if ((p < 0) != (i == 0)) return fail(FG_E_ARG, "every sequence's first row must be the root of its others");
+                depth[i] = p < 0 ? 1 : depth[p] + 1;
+                deepest = std::max(deepest, depth[i]);
+            }
+            if (ld < deepest) return fail(FG_E_SHAPE, "the outputs hold fewer tokens than the longest branch has rows");
+            rows += q.n;
+        }
+        // behind the plan: a parameter set and a uniform number per row, the outputs
+        const size_t o_prm = 0, o_u = o_prm + rows * 4, o_out = (o_u + rows + 63) / 64 * 64, o_path = o_out + (size_t)n_seqs * ld,
+                     o_cnt = o_path + (size_t)n_seqs * ld, more = o_cnt + n_seqs;
+        Plan P;
+        Work w{};
+        rc = tree_forward(
+            ctx, m, kv, seqs, n_seqs, P, w, more,
+            [&](int32_t* h) {
+                if (!sampling) return;
+                fg_sampling* pr = (fg_sampling*)(h + o_prm);
+                for (int s = 0; s < n_seqs; s++)
+                    for (int i = 0; i < seqs[s].n; i++) *pr++ = params[s];
+                memcpy(h + o_u, u, rows * 4);
+            },
+            sampling);
+        if (rc) return rc;
+        int32_t *dm = (int32_t*)ctx->dmeta, *dx = dm + P.words, *hx = (int32_t*)ctx->hmeta + P.words;
+        const RowArgs ra = row_args(P.rp, dm + P.o_rows);
+        const uint32_t* tokens = (const uint32_t*)(dm + P.o_tok);
+        hipStream_t st = ctx->stream;
+        if (sampling) {
+            const int V = m->cfg.vocab;
+            const size_t sb = (sample_bytes(P.S, wide, V) + 255) / 256 * 256;
+            if ((rc = ensure(&ctx->sbuf, &ctx->sbuf_cap, sb + (size_t)P.S * V * 4, st, false))) return rc;
+            SampleRows d = sample_rows(ctx->sbuf, P.S, 0, wide, V);
+            float* dense = (float*)((char*)ctx->sbuf + sb);
+            const SampleParams* prm = (const SampleParams*)(dx + o_prm);
+            launch_dist(st, w.logits, P.S, V, 1, prm, d);
+            launch_dense(st, d, P.S, prm, w.am, dense);
+            VerifyArgs v;
+            v.tokens = tokens;
+            v.p = dense;
+            v.u = (const float*)(dx + o_u);
+            v.vocab = V;
+            v.kind = DRAFT_FIXED;
+            v.out_tokens = (uint32_t*)(dx + o_out);
+            v.out_path = dx + o_path;
+            v.out_count = dx + o_cnt;
+            v.ld = ld;
+            launch_tree_verify(st, ra, v);
+        } else {
+            launch_tree_accept(st, ra, tokens, w.am, (uint32_t*)(dx + o_out), dx + o_path, dx + o_cnt, ld);
+        }
+        launch_kv_commit(st, ra, kv->layer(0), (int)m->layers.size(), kv->layer_bytes(), dx + o_path, dx + o_cnt, ld);
+        HIPCHK(hipGetLastError());
+        HIPCHK(hipMemcpyAsync(hx + o_out, dx + o_out, (more - o_out) * 4, hipMemcpyDeviceToHost, st));
+        HIPCHK(hipStreamSynchronize(st));
+        memcpy(out_tokens, hx + o_out, (size_t)n_seqs * ld * 4);
+        memcpy(out_path, hx + o_path, (size_t)n_seqs * ld * 4);
+        memcpy(out_count, hx + o_cnt, (size_t)n_seqs * 4);
+        return 0;
+    });
 }
 
 }  // extern "C"

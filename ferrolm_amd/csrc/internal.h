@@ -4,6 +4,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 namespace fg {
 
 // ---------------------------------------------------------------------------
@@ -345,5 +347,90 @@ void launch_sq_err(hipStream_t st, const float* y, int64_t ystride, int count, c
 constexpr int kStampSlots = 1024, kStampWgs = 1024;
 int stamps_read(uint64_t* out, int slots);
 int stamps_clear(hipStream_t st);
+
+// ---------------------------------------------------------------------------
+// Rows over paged caches (cache.hip, tree.hip, verify.hip): chains of tokens or
+// drafted trees, whose keys and values are quantized into the cache, which
+// attend to their context and their own branch, and which are verified.
+//
+// A block of an 8-bit cache holds, per head, 16 tokens of HD channels as
+//   K codes [16 tokens][HD], V codes [4 token groups][HD][4 tokens],
+//   16 K scales, 16 V scales (f32)
+// in 32 HD + 128 consecutive bytes: [layer][block][kv head][record]. A row's value is code * scale. The
+// layouts are those of the MFMA operands (k_tree_attn): a lane's keys are HD / 4 consecutive bytes, its
+// values HD / 4 too, and what a wave reads of a record is contiguous.
+// ---------------------------------------------------------------------------
+enum { KV_F32 = 0, KV_INT8 = 1, KV_FP8 = 2 };
+__host__ __device__ inline size_t kv_record(int hd) { return 32 * (size_t)hd + 128; }
+
+struct KvLayer {  // one layer of a cache
+    int format = 0, nkv = 0, hd = 0;
+    float *k = nullptr, *v = nullptr;  // KV_F32: [block][kv head][16][hd]
+    uint8_t* data = nullptr;           // 8-bit formats: [block][kv head][record]
+};
+
+// Device arrays of a set of rows (RowPlan in rows.h lays them out).
+constexpr int kSeqWords = 8;   // first row, rows, pos, first block in btab, first mask word (-1: a chain),
+                               // mask words per row, first token of the read-back, tokens cached
+constexpr int kItemWords = 8;  // sequence (-1: unused), first row, first and last page, first partial slot, slots
+                               // between the item's row slots, row slots, 1: no other item has these rows
+struct RowArgs {
+    const int32_t *seqs = nullptr, *btab = nullptr, *items = nullptr;
+    const int32_t* mrec = nullptr;   // per row: its first query in the slot, first partial slot, parts, 1: unused row
+    const int32_t* quads = nullptr;  // rows of one page's aligned group of four tokens: first row (its first
+                                     // token's, used or not), block, group, mask of the used tokens
+    const int32_t* rpos = nullptr;   // per row: its position on its branch
+    const uint16_t* masks = nullptr; // per row of a tree and page from pos / 16 on: tokens that it sees
+    const int32_t *cstart = nullptr, *clist = nullptr;  // children of each row, in order
+    int n_seqs = 0, rows = 0, n_items = 0, n_wi = 0, n_quads = 0, longest = 0, widest = 0;  // widest: most children of a row
+    bool unused = false, parts = false;  // some row is unused; some row has several items
+    int qt = 0, rw = 0, pw = 0;      // 16-query tiles a wave, row slots and position shares a workgroup
+};
+
+// Keys and values of the rows (k, v: [row][kv head][hd], ld floats between rows) into the cache. With
+// cos_t the keys are rotated first, by their row's position.
+int launch_kv_append(hipStream_t st, const RowArgs& a, const KvLayer& kv, const float* k, const float* v, int64_t ld,
+                     const float* cos_t, const float* sin_t);
+// The cached keys and values of the rows, or of every token of their sequences, in f32: [token][kv head][hd].
+int launch_kv_gather(hipStream_t st, const RowArgs& a, const KvLayer& kv, bool context, float* k, float* v);
+// A whole layer between the record layout and [block][kv head][16][hd] f32.
+int launch_kv_unpack(hipStream_t st, const KvLayer& kv, int blocks, float* k, float* v);
+int launch_kv_pack(hipStream_t st, const KvLayer& kv, int blocks, const float* k, const float* v);
+// Row path[s][j] of each sequence, j < count[s], to position pos + j, in every layer.
+int launch_kv_commit(hipStream_t st, const RowArgs& a, const KvLayer& first, int layers, size_t layer_bytes,
+                     const int32_t* path, const int32_t* count, int ld);
+
+struct TreeAttn {
+    const float* q = nullptr;  // [row][query head][hd], ldq floats between rows
+    int64_t ldq = 0;
+    float* out = nullptr;      // [row][query head][hd], ldo floats between rows; nullptr: partials only, for the merge
+    int64_t ldo = 0;           // kernels of the forward pass (AttnArgs::part, maxima in natural units)
+    float* part = nullptr;     // [partial slot][kv head][attn_qmax(hd)][hd + 4]
+    int nh = 0;
+    float scale = 0;
+    const float *cos_t = nullptr, *sin_t = nullptr;  // with them the queries are rotated first
+};
+int launch_tree_attn(hipStream_t st, const RowArgs& a, const KvLayer& kv, const TreeAttn& t);
+// The attention partials of launch_attention (or of launch_tree_attn without out) into pieces.
+int launch_merge(hipStream_t st, const AttnArgs& a, int m, int consumer_kind, Pieces& out);
+
+enum { DRAFT_EACH = 0, DRAFT_DISTINCT = 1, DRAFT_FIXED = 2 };
+struct VerifyArgs {
+    const uint32_t* tokens = nullptr;  // [row]
+    const float *p = nullptr, *q = nullptr;  // [row][vocab]
+    const float* u = nullptr;          // [row]: a first row's is its sequence's final draw, others' their test
+    int vocab = 0, kind = 0;
+    uint32_t* out_tokens = nullptr;    // [sequence][ld]
+    int32_t* out_path = nullptr;
+    int32_t* out_count = nullptr;      // [sequence]
+    int ld = 0;
+};
+void launch_tree_verify(hipStream_t st, const RowArgs& a, const VerifyArgs& v);
+// The greedy walk: the child whose token is its parent's argmax passes.
+void launch_tree_accept(hipStream_t st, const RowArgs& a, const uint32_t* tokens, const uint32_t* argmax,
+                        uint32_t* out_tokens, int32_t* out_path, int32_t* out_count, int ld);
+// Distributions of launch_dist (prm[row]) as dense rows [row][vocab]; a greedy row is all on its argmax.
+void launch_dense(hipStream_t st, const SampleRows& d, int rows, const SampleParams* prm, const uint32_t* argmax,
+                  float* p);
 
 }  // namespace fg

@@ -2557,34 +2557,8 @@ static void attn_ns(hipStream_t st, const AttnArgs& a) {
         hipLaunchKernelGGL((k_attn<HD, P, QM, 1, QL, MINW>), dim3(a.nkv, a.n_wi), dim3(256), 0, st, a);
 }
 
-template <int HD, int P, int QM>
-static void attention_hd(hipStream_t st, const AttnArgs& a, int m, int ck, Pieces& out) {
-    if constexpr ((HD == 64 || HD == 128) && QM == 32) {
-        if (a.flash) {
-            hipLaunchKernelGGL((k_attn_flash<HD, kFlashBlock(HD)>), dim3(a.nkv, a.n_wi / 2), dim3(256), 0, st, a);
-            goto merge;
-        }
-    }
-    // items of at most 8 or 24 queries hold fewer (three workgroups per CU);
-    // large launches of decode-sized items of one span at hd 64 and 128 keep
-    // their keys and values in registers (small ones: the general kernel's
-    // shorter chain of barriers finishes a lone item sooner)
-    if constexpr ((HD == 64 || HD == 128) && QM >= 8) {
-        if (a.ns == 1 && a.maxq > 0 && a.maxq <= 8 && (int64_t)a.nkv * a.n_wi >= kAttnDecWorkgroups) {
-            if (a.maxq <= 4)
-                hipLaunchKernelGGL((k_attn_dec<HD, P, QM, 4, 4>), dim3(a.nkv, a.n_wi), dim3(256), 0, st, a);
-            else
-                hipLaunchKernelGGL((k_attn_dec<HD, P, QM, 8, 4>), dim3(a.nkv, a.n_wi), dim3(256), 0, st, a);
-            goto merge;
-        }
-    }
-    if (QM > 8 && a.maxq > 0 && a.maxq <= 8)
-        attn_ns<HD, P, QM, 8, 3>(st, a);
-    else if (QM > 24 && a.maxq > 0 && a.maxq <= 24)
-        attn_ns<HD, P, QM, 24, 3>(st, a);
-    else
-        attn_ns<HD, P, QM, QM, 2>(st, a);
-merge:
+template <int HD, int QM>
+static void merge_hd(hipStream_t st, const AttnArgs& a, int m, int ck, Pieces& out) {
     if (ck < 0) return;  // the consumer merges the spans itself
     AttnArgs am = a;
     am.stamp = a.stamp >= 0 ? a.stamp + 1 : -1;  // the merge's timeline slot follows the attention's
@@ -2603,6 +2577,36 @@ merge:
     else
         hipLaunchKernelGGL((k_merge_pieces<HD, QM, INT8>), dim3(out.kb, out.passes), dim3(64), 0, st, am, m, out.a,
                            out.xs, out.passes);
+}
+
+template <int HD, int P, int QM>
+static void attention_hd(hipStream_t st, const AttnArgs& a, int m, int ck, Pieces& out) {
+    if constexpr ((HD == 64 || HD == 128) && QM == 32) {
+        if (a.flash) {
+            hipLaunchKernelGGL((k_attn_flash<HD, kFlashBlock(HD)>), dim3(a.nkv, a.n_wi / 2), dim3(256), 0, st, a);
+            return merge_hd<HD, QM>(st, a, m, ck, out);
+        }
+    }
+    // items of at most 8 or 24 queries hold fewer (three workgroups per CU);
+    // large launches of decode-sized items of one span at hd 64 and 128 keep
+    // their keys and values in registers (small ones: the general kernel's
+    // shorter chain of barriers finishes a lone item sooner)
+    if constexpr ((HD == 64 || HD == 128) && QM >= 8) {
+        if (a.ns == 1 && a.maxq > 0 && a.maxq <= 8 && (int64_t)a.nkv * a.n_wi >= kAttnDecWorkgroups) {
+            if (a.maxq <= 4)
+                hipLaunchKernelGGL((k_attn_dec<HD, P, QM, 4, 4>), dim3(a.nkv, a.n_wi), dim3(256), 0, st, a);
+            else
+                hipLaunchKernelGGL((k_attn_dec<HD, P, QM, 8, 4>), dim3(a.nkv, a.n_wi), dim3(256), 0, st, a);
+            return merge_hd<HD, QM>(st, a, m, ck, out);
+        }
+    }
+    if (QM > 8 && a.maxq > 0 && a.maxq <= 8)
+        attn_ns<HD, P, QM, 8, 3>(st, a);
+    else if (QM > 24 && a.maxq > 0 && a.maxq <= 24)
+        attn_ns<HD, P, QM, 24, 3>(st, a);
+    else
+        attn_ns<HD, P, QM, QM, 2>(st, a);
+    merge_hd<HD, QM>(st, a, m, ck, out);
 }
 
 int attn_span(int hd) { return hd >= 128 ? 32 : 64; }
@@ -2784,6 +2788,17 @@ int launch_attention(hipStream_t st, const AttnArgs& a, int m, int consumer_kind
         case 64: attention_hd<64, 64, 32>(st, a, m, consumer_kind, out); return 0;
         case 128: attention_hd<128, 32, 32>(st, a, m, consumer_kind, out); return 0;
         default: return -1;  // no instance: nothing is launched
+    }
+}
+
+int launch_merge(hipStream_t st, const AttnArgs& a, int m, int consumer_kind, Pieces& out) {
+    if (m <= 0 || a.n_wi <= 0) return 0;
+    switch (a.hd) {
+        case 16: merge_hd<16, 64>(st, a, m, consumer_kind, out); return 0;
+        case 32: merge_hd<32, 64>(st, a, m, consumer_kind, out); return 0;
+        case 64: merge_hd<64, 32>(st, a, m, consumer_kind, out); return 0;
+        case 128: merge_hd<128, 32>(st, a, m, consumer_kind, out); return 0;
+        default: return -1;
     }
 }
 

@@ -1,0 +1,219 @@
+// The host-side plan of a set of rows over a paged cache (RowArgs): which
+// tokens a row sees, how the attention is cut into items, which rows share a
+// page's group of four tokens, and the children of each drafted row. Host code
+// only.
+#pragma once
+#include "internal.h"
+
+#include <algorithm>
+#include <cstring>
+#include <vector>
+
+namespace fg {
+
+struct RowSeq {
+    int n = 0, pos = 0;
+    const uint32_t* blocks = nullptr;
+    int n_blocks = 0;
+    const int32_t* parents = nullptr;  // nullptr: a chain
+};
+
+// Longest tree: its masks hold a bit per row and token of the tree.
+constexpr int kTreeRows = 4096;
+// Workgroups that an attention launch is cut into where the context allows.
+constexpr int kTreeTarget = 512;
+
+struct RowPlan {
+    int n_seqs = 0, rows = 0, n_wi = 0, n_items = 0, n_quads = 0, longest = 0, deepest = 0, widest = 0;
+    uint32_t top_block = 0;  // the highest block id
+    int64_t tokens = 0;  // cached tokens of all sequences, rows among them
+    int qt = 1, rw = 1, pw = 1;
+    bool unused = false, parts = false;  // some row is unused; some row has several items
+    bool rooted = true;  // every sequence's rows hang on its first
+    std::vector<int32_t> seqs, btab, items, mrec, quads, rpos, cstart, clist;
+    std::vector<uint16_t> masks;
+    size_t o_seqs = 0, o_btab = 0, o_items = 0, o_mrec = 0, o_quads = 0, o_rpos = 0, o_masks = 0, o_cstart = 0,
+           o_clist = 0, words = 0;
+};
+
+// Checked by the caller: n >= 0, parents[i] in [-2, i), a block for every position.
+inline void plan_rows(RowPlan& P, const RowSeq* in, int n_seqs, int nh, int nkv, int hd, bool cached) {
+    P = RowPlan();
+    P.n_seqs = n_seqs;
+    const int G = std::max(1, nh / nkv), qm = attn_qmax(hd), rps = std::max(1, qm / G);  // rows of a slot
+    int most_q = 1, most_slots = 1;
+    for (int s = 0; s < n_seqs; s++) {
+        const RowSeq& q = in[s];
+        const int row0 = P.rows, L = q.pos + q.n, page0 = q.pos / 16, pages = (L + 15) / 16;
+        bool chain = true;
+        for (int i = 0; q.parents && i < q.n; i++) chain = chain && q.parents[i] == i - 1;
+        const int tp = chain ? 0 : pages - page0;
+        const int32_t rec[kSeqWords] = {row0, q.n, q.pos, (int32_t)P.btab.size(), chain ? -1 : (int32_t)P.masks.size(),
+                                        tp, (int32_t)P.tokens, L};
+        P.seqs.insert(P.seqs.end(), rec, rec + kSeqWords);
+        for (int b = 0; cached && b < pages; b++) {
+            P.btab.push_back((int32_t)q.blocks[b]);
+            P.top_block = std::max(P.top_block, q.blocks[b]);
+        }
+        // ancestors, depths, children
+        const int aw = (q.n + 63) / 64;
+        std::vector<uint64_t> anc(chain ? 0 : (size_t)q.n * aw, 0);
+        std::vector<int> depth(q.n), kids(q.n + 1, 0);
+        for (int i = 0; i < q.n; i++) {
+            const int p = chain ? i - 1 : q.parents[i];
+            depth[i] = p >= 0 ? depth[p] + 1 : 0;
+            if (p >= 0) kids[p + 1]++;
+            P.rooted = P.rooted && (i == 0 ? p == -1 : p != -1);
+            P.unused = P.unused || p == -2;
+            if (p != -2) P.deepest = std::max(P.deepest, depth[i] + 1);
+            P.rpos.push_back(q.pos + depth[i]);
+            if (chain || p == -2) continue;
+            uint64_t* a = &anc[(size_t)i * aw];
+            if (p >= 0) std::memcpy(a, &anc[(size_t)p * aw], aw * 8);
+            a[i / 64] |= 1ull << (i % 64);
+        }
+        P.rooted = P.rooted && q.n > 0;
+        for (int i = 0; i < q.n; i++) {
+            P.widest = std::max(P.widest, kids[i + 1]);
+            kids[i + 1] += kids[i];
+        }
+        const int c0 = (int)P.clist.size();
+        for (int i = 0; i < q.n; i++) P.cstart.push_back(c0 + kids[i]);
+        P.clist.resize(c0 + kids[q.n]);
+        for (int i = 0; i < q.n; i++) {
+            const int p = chain ? i - 1 : q.parents[i];
+            if (p >= 0) P.clist[c0 + kids[p]++] = row0 + i;
+        }
+        auto dead = [&](int i) { return !chain && q.parents[i] == -2; };
+        for (int i = 0; !chain && i < q.n; i++)
+            for (int x = 0; x < tp; x++) {
+                uint32_t m = 0;
+                for (int b = 0; b < 16 && !dead(i); b++) {
+                    const int j = (page0 + x) * 16 + b - q.pos;
+                    if (j < 0 || (j < q.n && (anc[(size_t)i * aw + j / 64] >> (j % 64) & 1))) m |= 1u << b;
+                }
+                P.masks.push_back((uint16_t)m);
+            }
+        // groups of four tokens
+        for (int t = q.pos / 4 * 4; cached && t < L; t += 4) {
+            int used = 0;
+            for (int b = 0; b < 4; b++)
+                if (t + b >= q.pos && t + b < L && !dead(t + b - q.pos)) used |= 1 << b;
+            if (!used) continue;
+            const int32_t qr[4] = {row0 + t - q.pos, (int32_t)q.blocks[t / 16], t % 16 / 4, used};
+            P.quads.insert(P.quads.end(), qr, qr + 4);
+        }
+        if (cached) P.n_quads += (q.n + 6) / 4;  // at most, wherever the rows start
+        for (int i = 0; i < q.n; i++) {
+            const int32_t mr[4] = {i % rps * G, 0, 0, dead(i) ? 1 : 0};
+            P.mrec.insert(P.mrec.end(), mr, mr + 4);
+        }
+        if (q.n) {
+            most_q = std::max(most_q, std::min(q.n, rps) * G);
+            most_slots = std::max(most_slots, (q.n + rps - 1) / rps);
+            P.longest = std::max(P.longest, L);
+        }
+        P.rows += q.n;
+        P.tokens += L;
+    }
+    P.cstart.push_back((int32_t)P.clist.size());
+    P.qt = most_q <= 16 ? 1 : qm / 16;
+    P.rw = std::min(4, most_slots);
+    P.pw = P.rw == 1 ? 8 : P.rw == 2 ? 4 : 2;
+    // items: rw slots of rows x a part of the pages that they see, in parts of even length
+    auto group_pages = [&](const RowSeq& q, int r0) {
+        const bool chain = P.seqs[(&q - in) * kSeqWords + 4] < 0;
+        const int last = chain ? q.pos + std::min(q.n, r0 + P.rw * rps) : q.pos + q.n;
+        return (last + 15) / 16;
+    };
+    int64_t work = 0;
+    for (int s = 0; cached && s < n_seqs; s++)
+        for (int r0 = 0; r0 < in[s].n; r0 += P.rw * rps) work += group_pages(in[s], r0);
+    const int step = 2 * P.pw;  // pages of one round of the workgroup's waves
+    int64_t len = (work * nkv + kTreeTarget - 1) / kTreeTarget;
+    len = std::max<int64_t>((len + step - 1) / step * step, step);
+    for (int s = 0; cached && s < n_seqs; s++)
+        for (int r0 = 0; r0 < in[s].n; r0 += P.rw * rps) {
+            const RowSeq& q = in[s];
+            const int pages = group_pages(q, r0), parts = (int)((pages + len - 1) / len);
+            const int per = ((pages + parts - 1) / parts + step - 1) / step * step;
+            const int np = (pages + per - 1) / per, slots = std::min(P.rw, (q.n - r0 + rps - 1) / rps);
+            for (int p = 0; p < np; p++) {
+                const int32_t rec[kItemWords] = {s, r0, p * per, std::min(pages, (p + 1) * per), P.n_wi + p, np, slots,
+                                                 np == 1};
+                P.items.insert(P.items.end(), rec, rec + kItemWords);
+                P.n_items++;
+            }
+            for (int i = r0; i < std::min(q.n, r0 + P.rw * rps); i++) {
+                int32_t* mr = &P.mrec[(size_t)(P.seqs[s * kSeqWords] + i) * 4];
+                mr[1] = P.n_wi + (i - r0) / rps * np;
+                mr[2] = np;
+            }
+            P.parts = P.parts || np > 1;
+            P.n_wi += np * slots;
+        }
+    auto place = [&](size_t n) {
+        const size_t r = P.words;
+        P.words += (n + 63) / 64 * 64;
+        return r;
+    };
+    // capacities in steps, so that the layout (and a captured step) lasts while contexts grow; the
+    // added items and quads are unused
+    P.n_items = (P.n_items + 15) / 16 * 16;
+    P.items.resize((size_t)P.n_items * kItemWords, -1);
+    P.quads.resize((size_t)P.n_quads * 4, 0);
+    P.n_wi = (P.n_wi + 15) / 16 * 16;
+    P.btab.resize((P.btab.size() + 255) / 256 * 256, 0);
+    P.o_seqs = place(P.seqs.size());
+    P.o_btab = place(P.btab.size());
+    P.o_items = place(P.items.size());
+    P.o_mrec = place(P.mrec.size());
+    P.o_quads = place(P.quads.size());
+    P.o_rpos = place(P.rpos.size());
+    P.o_masks = place((P.masks.size() + 1) / 2);
+    P.o_cstart = place(P.cstart.size());
+    P.o_clist = place(P.clist.size());
+}
+
+inline void pack_rows(const RowPlan& P, int32_t* h) {
+    auto cp = [&](size_t off, const std::vector<int32_t>& v) {
+        if (!v.empty()) std::memcpy(h + off, v.data(), v.size() * 4);
+    };
+    cp(P.o_seqs, P.seqs);
+    cp(P.o_btab, P.btab);
+    cp(P.o_items, P.items);
+    cp(P.o_mrec, P.mrec);
+    cp(P.o_quads, P.quads);
+    cp(P.o_rpos, P.rpos);
+    cp(P.o_cstart, P.cstart);
+    cp(P.o_clist, P.clist);
+    if (!P.masks.empty()) std::memcpy(h + P.o_masks, P.masks.data(), P.masks.size() * 2);
+}
+
+inline RowArgs row_args(const RowPlan& P, const int32_t* d) {
+    RowArgs a;
+    a.seqs = d + P.o_seqs;
+    a.btab = d + P.o_btab;
+    a.items = d + P.o_items;
+    a.mrec = d + P.o_mrec;
+    a.quads = d + P.o_quads;
+    a.rpos = d + P.o_rpos;
+    a.masks = (const uint16_t*)(d + P.o_masks);
+    a.cstart = d + P.o_cstart;
+    a.clist = d + P.o_clist;
+    a.n_seqs = P.n_seqs;
+    a.rows = P.rows;
+    a.n_items = P.n_items;
+    a.n_wi = P.n_wi;
+    a.n_quads = P.n_quads;
+    a.longest = P.longest;
+    a.widest = P.widest;
+    a.unused = P.unused;
+    a.parts = P.parts;
+    a.qt = P.qt;
+    a.rw = P.rw;
+    a.pw = P.pw;
+    return a;
+}
+
+}  // namespace fg

@@ -1,0 +1,572 @@
+// Attention of rows over a paged cache: chains, single tokens and trees of
+// drafted tokens, over f32, int8 and fp8 caches.
+//
+// Row i of a sequence with `pos` cached tokens before its rows attends to
+// those and to its own branch: o = sum_t softmax_t(q . k_t / sqrt(HD)) v_t,
+// one pass with a running maximum m and sum l per query.
+//
+// A wave holds up to 16 QT queries (rows x grouped heads, a slot) of one kv
+// head and takes pairs of pages. Both products run transposed on f16 MFMA
+// (16x16x32): scores K q^T leave a lane with one query and four tokens of each
+// page, which is the operand layout of V^T p^T, so scores and probabilities
+// never leave their registers, and all of a query's state sits in its lanes.
+// The cache's records are in operand layout (internal.h): loads go from memory
+// to registers, with no LDS and no barrier before the shares of a workgroup's
+// waves meet.
+//
+// Precision: int8 and fp8 codes are exact in f16. Queries are scaled by a power
+// of two and split into two f16, to 2^-21 of each input and 2^-31 of the
+// largest; probabilities times value scales likewise. f32 keys and values are
+// scaled by row and split the same way (the product of the two small parts,
+// 2^-22, is left out). Sums are f32.
+#include "devutil.h"
+
+namespace fg {
+
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+
+namespace {
+
+constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
+// Below every score; its exponential is 0 against any.
+constexpr float kLowest = -1e30f;
+
+// Eight codes, of which d0 holds the first four, in f16.
+template <int FMT>
+__device__ __forceinline__ f16x8 codes8(uint32_t d0, uint32_t d1) {
+    uint32_t h[4];
+    if constexpr (FMT == KV_INT8) {
+        // 0x6400 | (code + 128) is 1152 + code as f16
+        const uint32_t x0 = d0 ^ 0x80808080u, x1 = d1 ^ 0x80808080u;
+        h[0] = __builtin_amdgcn_perm(0x64646464u, x0, 0x04010400u);
+        h[1] = __builtin_amdgcn_perm(0x64646464u, x0, 0x04030402u);
+        h[2] = __builtin_amdgcn_perm(0x64646464u, x1, 0x04010400u);
+        h[3] = __builtin_amdgcn_perm(0x64646464u, x1, 0x04030402u);
+        f16x8 r;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const f16x2 y = __builtin_bit_cast(f16x2, h[i]) - (f16x2){(_Float16)1152.0f, (_Float16)1152.0f};
+            r[2 * i] = y[0];
+            r[2 * i + 1] = y[1];
+        }
+        return r;
+    } else {
+        f16x8 r;
+        const f16x2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(d0, 1.0f, false),
+                    b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(d0, 1.0f, true),
+                    c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(d1, 1.0f, false),
+                    d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(d1, 1.0f, true);
+        r[0] = a[0], r[1] = a[1], r[2] = b[0], r[3] = b[1], r[4] = c[0], r[5] = c[1], r[6] = d[0], r[7] = d[1];
+        return r;
+    }
+}
+
+__device__ __forceinline__ f32x4 mfma(f16x8 a, f16x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
+// x = hi + lo, rounded towards zero: to 2^-21 of x, or 2^-24 where that is more (f16's smallest step)
+__device__ __forceinline__ void split2(float x0, float x1, uint32_t& hi, uint32_t& lo) {
+    const auto h = __builtin_amdgcn_cvt_pkrtz(x0, x1);
+    hi = __builtin_bit_cast(uint32_t, h);
+    const f16x2 f = __builtin_bit_cast(f16x2, hi);
+    lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x0 - (float)f[0], x1 - (float)f[1]));
+}
+__device__ __forceinline__ void split8(const float (&x)[8], f16x8& hi, f16x8& lo) {
+    u32x4 h, l;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        uint32_t a, b;
+        split2(x[2 * i], x[2 * i + 1], a, b);
+        h[i] = a, l[i] = b;
+    }
+    hi = __builtin_bit_cast(f16x8, h);
+    lo = __builtin_bit_cast(f16x8, l);
+}
+
+// The exponent that brings values up to m below 2^6 (the two halves then hold them to 2^-31 of m, their products
+// far from f32's ends); bounded, so that 2^-e stays finite.
+__device__ __forceinline__ int split_exp(float m) {
+    int e = 0;
+    if (m > 0.0f && m < INFINITY) frexpf(m, &e);
+    return max(e, -100) - 6;
+}
+
+// What a lane takes of a page: keys of token lane % 16 at channels (lane / 16) HD / 4 .., values of tokens
+// 4 (lane / 16) .. +3 at channels (lane % 16) HD / 16 .., and the scales of those four tokens.
+template <int HD, int FMT>
+struct Page {
+    static constexpr int KD = HD / 16;
+    uint32_t k[KD], v[KD];
+    float4 ks, vs;
+    template <class T>
+    static __device__ __forceinline__ void words(const uint8_t* p, T* d) {
+        if constexpr (KD == 1) {
+            d[0] = *(const uint32_t*)p;
+        } else if constexpr (KD == 2) {
+            const u32x2 x = *(const u32x2*)p;
+            d[0] = x[0], d[1] = x[1];
+        } else {
+#pragma unroll
+            for (int i = 0; i < KD / 4; i++) {
+                const u32x4 x = *(const u32x4*)(p + 16 * i);
+#pragma unroll
+                for (int e = 0; e < 4; e++) d[4 * i + e] = x[e];
+            }
+        }
+    }
+    __device__ __forceinline__ void load(const KvLayer& kv, size_t block, int h, int lane) {
+        const uint8_t* rec = kv.data + (block * kv.nkv + h) * kv_record(HD);
+        const int r = lane & 15, g = lane >> 4;
+        words(rec + r * HD + g * (HD / 4), k);
+        words(rec + 16 * HD + g * (4 * HD) + r * (HD / 4), v);
+        ks = *(const float4*)(rec + 32 * HD + 16 * g);
+        vs = *(const float4*)(rec + 32 * HD + 64 + 16 * g);
+    }
+};
+template <int HD>
+struct Page<HD, KV_F32> {
+    static constexpr int N = HD / 4, C = HD / 16;  // a lane's key channels; its value channels of each of four tokens
+    float k[N], v[4][C];
+    __device__ __forceinline__ void load(const KvLayer& kv, size_t block, int h, int lane) {
+        const size_t at = (block * kv.nkv + h) * 16 * HD;
+        const int r = lane & 15, g = lane >> 4;
+        const float* kp = kv.k + at + r * HD + g * N;
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+            const float4 x = *(const float4*)(kp + i);
+            k[i] = x.x, k[i + 1] = x.y, k[i + 2] = x.z, k[i + 3] = x.w;
+        }
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            const float* vp = kv.v + at + (4 * g + t) * HD + r * C;
+            if constexpr (C >= 4) {
+#pragma unroll
+                for (int i = 0; i < C; i += 4) {
+                    const float4 x = *(const float4*)(vp + i);
+                    v[t][i] = x.x, v[t][i + 1] = x.y, v[t][i + 2] = x.z, v[t][i + 3] = x.w;
+                }
+            } else if constexpr (C == 2) {
+                const float2 x = *(const float2*)vp;
+                v[t][0] = x.x, v[t][1] = x.y;
+            } else {
+                v[t][0] = *vp;
+            }
+        }
+    }
+};
+
+// A page as MFMA operands: the scores' key operand by steps of 32 channels, and the scales of the lane's four
+// tokens. lo is there for f32 caches only.
+template <int HD, int FMT>
+struct Keys {
+    static constexpr int NS = HD >= 32 ? HD / 32 : 1;
+    f16x8 hi[NS], lo[FMT == KV_F32 ? NS : 1];
+    float s[4];
+};
+
+template <int HD, int FMT>
+__device__ __forceinline__ void make_keys(const Page<HD, FMT>& p, Keys<HD, FMT>& o, int lane) {
+    if constexpr (FMT == KV_F32) {
+        float m = 0.0f;
+#pragma unroll
+        for (int i = 0; i < HD / 4; i++) m = fmaxf(m, fabsf(p.k[i]) <= 3.4e38f ? fabsf(p.k[i]) : INFINITY);
+        m = reduce_rows<true, true>(m);
+        const bool fine = m < INFINITY;
+        const int e = split_exp(m);
+        const float f = ldexpf(1.0f, -e);
+        const float sc = fine ? ldexpf(1.0f, e) : NAN;  // of key lane % 16
+#pragma unroll
+        for (int s = 0; s < Keys<HD, FMT>::NS; s++) {
+            float x[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[i] = 8 * s + i < HD / 4 && fine ? p.k[(8 * s + i) % (HD / 4)] * f : 0.0f;
+            split8(x, o.hi[s], o.lo[s]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) o.s[i] = __shfl(sc, 4 * (lane >> 4) + i);
+    } else {
+#pragma unroll
+        for (int s = 0; s < Keys<HD, FMT>::NS; s++)
+            o.hi[s] = codes8<FMT>(p.k[(2 * s) % (HD / 16)], HD >= 32 ? p.k[(2 * s + 1) % (HD / 16)] : 0u);
+        if constexpr (HD == 16) {  // only four channels a lane: the operand's other half is zero
+#pragma unroll
+            for (int i = 4; i < 8; i++) o.hi[0][i] = (_Float16)0.0f;
+        }
+        o.s[0] = p.ks.x, o.s[1] = p.ks.y, o.s[2] = p.ks.z, o.s[3] = p.ks.w;
+    }
+}
+
+// Scales of the lane's four values of a page, and for f32 the exponent to split them by.
+template <int HD, int FMT>
+__device__ __forceinline__ void value_scales(const Page<HD, FMT>& p, float (&s)[4], float (&f)[4]) {
+    if constexpr (FMT == KV_F32) {
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            float m = 0.0f;
+#pragma unroll
+            for (int i = 0; i < HD / 16; i++) m = fmaxf(m, fabsf(p.v[t][i]) <= 3.4e38f ? fabsf(p.v[t][i]) : INFINITY);
+            m = group_reduce<16, true>(m);
+            const int e = split_exp(m);
+            s[t] = m < INFINITY ? ldexpf(1.0f, e) : NAN;
+            f[t] = m < INFINITY ? ldexpf(1.0f, -e) : 0.0f;
+        }
+    } else {
+        s[0] = p.vs.x, s[1] = p.vs.y, s[2] = p.vs.z, s[3] = p.vs.w;
+    }
+}
+
+}  // namespace
+
+// One workgroup per (kv head, item): rw row slots x pw position shares, a wave
+// each; the shares' sums meet in LDS.
+template <int HD, int FMT, int QT>
+__global__ __launch_bounds__(512) void k_tree_attn(RowArgs a, KvLayer kv, TreeAttn t) {
+    constexpr int KD = HD / 16, NS = Keys<HD, FMT>::NS;
+    constexpr int QM = HD >= 64 ? 32 : 64;
+    constexpr bool F32 = FMT == KV_F32;
+    constexpr int ND = 4 * KD + 3;  // dwords a lane keeps of a tile
+    extern __shared__ float sh[];
+    const int h = blockIdx.x % kv.nkv, item = blockIdx.x / kv.nkv;
+    const int4 i0 = *(const int4*)(a.items + (size_t)item * kItemWords),
+               i1 = *(const int4*)(a.items + (size_t)item * kItemWords + 4);
+    if (i0.x < 0) return;  // an unused item of the launch's capacity
+    const int4 s0 = *(const int4*)(a.seqs + (size_t)i0.x * kSeqWords), s1 = *(const int4*)(a.seqs + (size_t)i0.x * kSeqWords + 4);
+    const int seq0 = s0.x, n = s0.y, pos = s0.z, btab = s0.w, mask0 = s1.x, mpages = s1.y;
+    const bool chain = mask0 < 0;
+    const int G = t.nh / kv.nkv, rps = QM / G;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
+    const int slot = wave % a.rw, share = wave / a.rw;
+    const int r0 = i0.y + slot * rps, nr = min(rps, n - r0), Q = nr * G;
+    const bool on = slot < i1.z && nr > 0;
+
+    f16x8 qh[QT][NS], ql[QT][NS];
+    // score factor; running maximum (log 2 units) and sum; the power of two at or above the value scales so far (a
+    // weight is the probability times the value scale over it, in [0, 1], times 2^13 for the split), 2^13 over it
+    float qf[QT], mq[QT], l[QT], ec[QT], vn[QT];
+    int qrow[QT];                          // the query's row in its sequence
+    f32x4 o[QT][KD];
+#pragma unroll
+    for (int i = 0; i < QT; i++) {
+        mq[i] = kLowest;
+        l[i] = 0.0f;
+        ec[i] = 0x1p-100f;
+        vn[i] = 0x1p113f;
+        qf[i] = 1.0f;
+        qrow[i] = 0;
+#pragma unroll
+        for (int j = 0; j < KD; j++) o[i][j] = (f32x4){0, 0, 0, 0};
+    }
+    if (on) {
+#pragma unroll
+        for (int i = 0; i < QT; i++) {
+            const int qi = min(16 * i + r, Q - 1);  // lanes past the last query hold it again
+            qrow[i] = r0 + qi / G;
+            const int64_t row = seq0 + qrow[i];
+            const float* qp = t.q + row * t.ldq + (h * G + qi % G) * HD;
+            float x[HD / 4];
+#pragma unroll
+            for (int e = 0; e < HD / 4; e += 4) {
+                const float4 w = *(const float4*)(qp + g * (HD / 4) + e);
+                x[e] = w.x, x[e + 1] = w.y, x[e + 2] = w.z, x[e + 3] = w.w;
+            }
+            if (t.cos_t) {  // rotate-half, src/model.rs:451-459
+                const float* cp = t.cos_t + (size_t)a.rpos[row] * (HD / 2) + (g & 1) * (HD / 4);
+                const float* sp = t.sin_t + (size_t)a.rpos[row] * (HD / 2) + (g & 1) * (HD / 4);
+#pragma unroll
+                for (int e = 0; e < HD / 4; e++) {
+                    const float y = qp[(g ^ 2) * (HD / 4) + e];
+                    x[e] = __fadd_rn(__fmul_rn(x[e], cp[e]), __fmul_rn(g < 2 ? -y : y, sp[e]));
+                }
+            }
+            float m = 0.0f;
+#pragma unroll
+            for (int e = 0; e < HD / 4; e++) m = fmaxf(m, fabsf(x[e]) <= 3.4e38f ? fabsf(x[e]) : INFINITY);
+            m = reduce_rows<true, true>(m);
+            const int ex = split_exp(m);
+            const float f = m < INFINITY ? ldexpf(1.0f, -ex) : NAN;
+            qf[i] = ldexpf(t.scale * kLog2e, ex);
+#pragma unroll
+            for (int s = 0; s < NS; s++) {
+                float y[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) y[e] = 8 * s + e < HD / 4 ? x[(8 * s + e) % (HD / 4)] * f : 0.0f;
+                split8(y, qh[i][s], ql[i][s]);
+            }
+        }
+        const int last = chain ? min(i0.w, (pos + r0 + nr + 15) / 16) : i0.w;  // pages that the slot's rows see
+        const int pairs = (last - i0.z + 1) / 2, mine = (pairs - share + a.pw - 1) / a.pw;
+        const int full = chain ? pos + r0 + 1 : pos;  // tokens that all of the slot's rows see
+        for (int c0 = 0; c0 < mine; c0 += 32) {
+            // the chunk's block ids, two pages a pair; past the last page the last again
+            const int pg = i0.z + 2 * (share + a.pw * (c0 + lane / 2)) + (lane & 1);
+            const int ids = a.btab[btab + min(pg, last - 1)];
+            const int np = min(32, mine - c0);
+            for (int c = 0; c < np; c++) {
+                const int p0 = i0.z + 2 * (share + a.pw * (c0 + c));  // the pair's first page
+                Page<HD, FMT> pg2[2];
+#pragma unroll
+                for (int x = 0; x < 2; x++)
+                    pg2[x].load(kv, (size_t)(uint32_t)__builtin_amdgcn_readlane(ids, 2 * c + x), h, lane);
+                float raw[2][QT][4], vsc[2][4], vf[2][4];
+#pragma unroll
+                for (int x = 0; x < 2; x++) {
+                    Keys<HD, FMT> k;
+                    make_keys<HD, FMT>(pg2[x], k, lane);
+                    value_scales<HD, FMT>(pg2[x], vsc[x], vf[x]);
+#pragma unroll
+                    for (int i = 0; i < QT; i++) {
+                        f32x4 acc = (f32x4){0, 0, 0, 0};
+#pragma unroll
+                        for (int s = 0; s < NS; s++) {
+                            acc = mfma(k.hi[s], ql[i][s], acc);
+                            if constexpr (F32) acc = mfma(k.lo[s], qh[i][s], acc);
+                            acc = mfma(k.hi[s], qh[i][s], acc);
+                        }
+#pragma unroll
+                        for (int e = 0; e < 4; e++) raw[x][i][e] = acc[e] * k.s[e];
+                    }
+                }
+                const bool masked = 16 * (p0 + 2) > full || p0 + 1 >= last;
+                float vmax = 0.0f;
+                if (masked) {
+#pragma unroll
+                    for (int x = 0; x < 2; x++)
+#pragma unroll
+                        for (int i = 0; i < QT; i++) {
+                            const int page = p0 + x, at = 16 * page + 4 * g;
+                            uint32_t sees = page < last ? 15u : 0u;
+                            if (chain)
+                                sees &= at > pos + qrow[i] ? 0u : 15u >> max(0, 3 - (pos + qrow[i] - at));
+                            else if (page >= pos / 16 && page < last)
+                                sees &= (uint32_t)a.masks[mask0 + (size_t)qrow[i] * mpages + (page - pos / 16)] >> (4 * g);
+#pragma unroll
+                            for (int e = 0; e < 4; e++) raw[x][i][e] = sees >> e & 1 ? raw[x][i][e] : -INFINITY;
+                        }
+                } else {
+#pragma unroll
+                    for (int x = 0; x < 2; x++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) vmax = fmaxf(vmax, vsc[x][e]);
+                    vmax = reduce_rows<true, true>(vmax);
+                }
+                uint32_t ph[QT][4], pl[QT][4];
+#pragma unroll
+                for (int i = 0; i < QT; i++) {
+                    float mx = -INFINITY, vm = vmax;
+#pragma unroll
+                    for (int x = 0; x < 2; x++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            mx = fmaxf(mx, raw[x][i][e]);
+                            if (masked && raw[x][i][e] != -INFINITY) vm = fmaxf(vm, vsc[x][e]);
+                        }
+                    mx = reduce_rows<true, true>(mx);
+                    if (masked) vm = reduce_rows<true, true>(vm);
+                    const float mn = fmaxf(mq[i], mx * qf[i]);
+                    // the power of two at or above the largest value scale
+                    const float en = fmaxf(ec[i], __uint_as_float((__float_as_uint(vm) + 0x7FFFFFu) & 0x7F800000u));
+                    if (__any(mn > mq[i] || en > ec[i])) {
+                        const float f = __builtin_amdgcn_exp2f(mq[i] - mn), fo = f * (ec[i] / en);
+                        l[i] *= f;
+#pragma unroll
+                        for (int j = 0; j < KD; j++) o[i][j] *= fo;
+                        mq[i] = mn;
+                        ec[i] = en;
+                        vn[i] = 8192.0f / en;
+                    }
+                    float w[8];
+#pragma unroll
+                    for (int x = 0; x < 2; x++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const float p = __builtin_amdgcn_exp2f(fmaf(raw[x][i][e], qf[i], -mq[i]));
+                            l[i] += p;
+                            w[4 * x + e] = masked && raw[x][i][e] == -INFINITY ? 0.0f : p * (vsc[x][e] * vn[i]);
+                        }
+#pragma unroll
+                    for (int e = 0; e < 4; e++) split2(w[2 * e], w[2 * e + 1], ph[i][e], pl[i][e]);
+                }
+#pragma unroll
+                for (int j = 0; j < KD; j++) {
+                    f16x8 vh, vl;
+                    if constexpr (F32) {
+                        float y[8];
+#pragma unroll
+                        for (int x = 0; x < 2; x++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) y[4 * x + e] = vf[x][e] == 0.0f ? 0.0f : pg2[x].v[e][j] * vf[x][e];
+                        split8(y, vh, vl);
+                    } else {
+                        vh = codes8<FMT>(pg2[0].v[j], pg2[1].v[j]);
+                    }
+#pragma unroll
+                    for (int i = 0; i < QT; i++) {
+                        const f16x8 hi = __builtin_bit_cast(f16x8, (u32x4){ph[i][0], ph[i][1], ph[i][2], ph[i][3]});
+                        const f16x8 lo = __builtin_bit_cast(f16x8, (u32x4){pl[i][0], pl[i][1], pl[i][2], pl[i][3]});
+                        o[i][j] = mfma(vh, lo, o[i][j]);
+                        if constexpr (F32) o[i][j] = mfma(vl, hi, o[i][j]);
+                        o[i][j] = mfma(vh, hi, o[i][j]);
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < QT; i++) l[i] = reduce_rows<false, true>(l[i]);
+    }
+    // the position shares, halved until one holds the sums; a tile at a time, for the LDS that takes
+    for (int half = a.pw / 2; half > 0; half >>= 1) {
+        float* x = sh + ((size_t)(share % half * a.rw + slot) * ND) * 64 + lane;
+#pragma unroll
+        for (int i = 0; i < QT; i++) {
+            if (on && share >= half && share < 2 * half) {
+                x[0] = mq[i];
+                x[64] = l[i];
+                x[128] = ec[i];
+#pragma unroll
+                for (int j = 0; j < KD; j++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) x[(3 + 4 * j + e) * 64] = o[i][j][e];
+            }
+            __syncthreads();
+            if (on && share < half) {
+                const float m2 = x[0], mn = fmaxf(mq[i], m2), en = fmaxf(ec[i], x[128]);
+                const float f1 = __builtin_amdgcn_exp2f(mq[i] - mn), f2 = __builtin_amdgcn_exp2f(m2 - mn);
+                const float w1 = f1 * (ec[i] / en), w2 = f2 * (x[128] / en);
+                l[i] = l[i] * f1 + x[64] * f2;
+#pragma unroll
+                for (int j = 0; j < KD; j++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) o[i][j][e] = o[i][j][e] * w1 + x[(3 + 4 * j + e) * 64] * w2;
+                mq[i] = mn;
+                ec[i] = en;
+            }
+            __syncthreads();
+        }
+    }
+    if (!on || share != 0) return;
+#pragma unroll
+    for (int i = 0; i < QT; i++) {
+        const int qi = 16 * i + r;
+        if (qi >= Q) continue;
+        const float sc = ec[i] * (1.0f / 8192.0f);
+        float* dst;
+        float f = sc;
+        if (t.out && i1.w) {
+            // no other item has these rows: what they attend to, zeros where that is nothing
+            const bool none = l[i] == 0.0f || a.mrec[(size_t)(seq0 + qrow[i]) * 4 + 3];
+            f = none ? 0.0f : sc / l[i];
+            if (none) {
+#pragma unroll
+                for (int j = 0; j < KD; j++) o[i][j] = (f32x4){0, 0, 0, 0};
+            }
+            dst = t.out + (size_t)(seq0 + qrow[i]) * t.ldo + (size_t)(h * G + qi % G) * HD;
+        } else {
+            float* part = t.part + (((size_t)(i1.x + slot * i1.y) * kv.nkv + h) * QM + qi) * (HD + 4);
+            if (g == 0) {
+                part[0] = l[i] == 0.0f ? -INFINITY : t.out ? mq[i] : mq[i] * kLn2;
+                part[1] = l[i];
+            }
+            dst = part + 4;
+        }
+        dst += g * (HD / 4);
+#pragma unroll
+        for (int w = 0; w < KD; w++) {  // channel 4 w + e of the lane's: tile (4 w + e) % KD, register (4 w + e) / KD
+            f32x4 y;
+#pragma unroll
+            for (int e = 0; e < 4; e++) y[e] = o[i][(4 * w + e) % KD][(4 * w + e) / KD] * f;
+            *(f32x4*)(dst + 4 * w) = y;
+        }
+    }
+}
+
+// The parts of each row's heads: one workgroup per (row, kv head x QH heads),
+// 4 channels a thread, the parts dealt over the rest of the workgroup's threads.
+template <int HD>
+__global__ __launch_bounds__(256) void k_tree_merge(RowArgs a, TreeAttn t, int nkv) {
+    constexpr int T = HD / 4, NP = 256 / T, QM = HD >= 64 ? 32 : 64;
+    __shared__ float4 so[NP][T];
+    __shared__ float sm[NP], sl[NP];
+    const int row = blockIdx.x, hq = blockIdx.y, G = t.nh / nkv, h = hq / G;
+    const int4 mr = *(const int4*)(a.mrec + (size_t)row * 4);
+    if (mr.z == 1) return;  // written by the attention
+    const int d = threadIdx.x % T, w = threadIdx.x / T;
+    const size_t stride = (size_t)nkv * QM * (HD + 4);
+    const float* base = t.part + (((size_t)mr.y * nkv + h) * QM + mr.x + hq % G) * (HD + 4);
+    float m = kLowest, l = 0.0f;
+    float4 o = make_float4(0, 0, 0, 0);
+    for (int s = w; s < mr.z; s += NP) {
+        const float* p = base + s * stride;
+        const float2 st = *(const float2*)p;
+        const float4 v = *(const float4*)(p + 4 + 4 * d);
+        if (st.x == -INFINITY) continue;
+        const float mn = fmaxf(m, st.x), f1 = __builtin_amdgcn_exp2f(m - mn), f2 = __builtin_amdgcn_exp2f(st.x - mn);
+        l = l * f1 + st.y * f2;
+        o.x = o.x * f1 + v.x * f2;
+        o.y = o.y * f1 + v.y * f2;
+        o.z = o.z * f1 + v.z * f2;
+        o.w = o.w * f1 + v.w * f2;
+        m = mn;
+    }
+    so[w][d] = o;
+    if (d == 0) {
+        sm[w] = m;
+        sl[w] = l;
+    }
+    __syncthreads();
+    if (w > 0) return;
+    const int np = min(NP, mr.z);
+    float M = kLowest, L = 0.0f;
+    for (int i = 0; i < np; i++) M = fmaxf(M, sm[i]);
+    float4 y = make_float4(0, 0, 0, 0);
+    for (int i = 0; i < np; i++) {
+        const float f = __builtin_amdgcn_exp2f(sm[i] - M);
+        const float4 v = so[i][d];
+        L += sl[i] * f;
+        y.x += v.x * f;
+        y.y += v.y * f;
+        y.z += v.z * f;
+        y.w += v.w * f;
+    }
+    const bool none = L == 0.0f || mr.w;
+    const float f = 1.0f / L;
+    y = none ? make_float4(0, 0, 0, 0) : make_float4(y.x * f, y.y * f, y.z * f, y.w * f);
+    *(float4*)(t.out + (size_t)row * t.ldo + (size_t)hq * HD + 4 * d) = y;
+}
+
+template <int HD, int FMT>
+static void tree_qt(hipStream_t st, const RowArgs& a, const KvLayer& kv, const TreeAttn& t) {
+    const dim3 grid((unsigned)kv.nkv * a.n_items), block(64 * a.rw * a.pw);
+    const size_t per = (size_t)64 * 4 * (4 * (HD / 16) + 3) * (a.pw / 2) * a.rw;
+    constexpr int QT = HD >= 64 ? 2 : 4;
+    if (a.qt == 1)
+        hipLaunchKernelGGL((k_tree_attn<HD, FMT, 1>), grid, block, per, st, a, kv, t);
+    else
+        hipLaunchKernelGGL((k_tree_attn<HD, FMT, QT>), grid, block, per, st, a, kv, t);
+}
+
+template <int HD>
+static void tree_hd(hipStream_t st, const RowArgs& a, const KvLayer& kv, const TreeAttn& t) {
+    if (kv.format == KV_F32)
+        tree_qt<HD, KV_F32>(st, a, kv, t);
+    else if (kv.format == KV_INT8)
+        tree_qt<HD, KV_INT8>(st, a, kv, t);
+    else
+        tree_qt<HD, KV_FP8>(st, a, kv, t);
+    if (t.out && a.parts) hipLaunchKernelGGL((k_tree_merge<HD>), dim3(a.rows, t.nh), dim3(256), 0, st, a, t, kv.nkv);
+}
+
+int launch_tree_attn(hipStream_t st, const RowArgs& a, const KvLayer& kv, const TreeAttn& t) {
+    if (a.rows <= 0) return 0;
+    switch (kv.hd) {
+        case 16: tree_hd<16>(st, a, kv, t); return 0;
+        case 32: tree_hd<32>(st, a, kv, t); return 0;
+        case 64: tree_hd<64>(st, a, kv, t); return 0;
+        case 128: tree_hd<128>(st, a, kv, t); return 0;
+        default: return -1;
+    }
+}
+
+}  // namespace fg

@@ -58,6 +58,11 @@ class FgSpecSeq(C.Structure):
                 ("blocks", u32p), ("n_blocks", C.c_int32), ("draft_blocks", u32p), ("n_draft_blocks", C.c_int32)]
 
 
+class FgTreeSeq(C.Structure):
+    _fields_ = [("tokens", u32p), ("n", C.c_int32), ("pos", C.c_int32), ("blocks", u32p), ("n_blocks", C.c_int32),
+                ("_pad", C.c_int32), ("parents", i32p)]
+
+
 class FgSampling(C.Structure):
     _fields_ = [("temperature", C.c_float), ("top_p", C.c_float), ("top_k", C.c_int32), ("reserved", C.c_int32)]
 
@@ -134,6 +139,24 @@ EXPORTS = {
     "fg_matmul_device": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p]),
     "fg_matmul_device_noalloc": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p]),
     "fg_mm_tile": (C.c_int, [C.c_int32] * 5 + [i32p] * 3),
+    "fg_ctx_wait_stream": (C.c_int, [C.c_void_p, C.c_void_p]),
+    "fg_stream_wait_ctx": (C.c_int, [C.c_void_p, C.c_void_p]),
+    "fg_kv_create_format": (C.c_int, [C.c_void_p] + [C.c_int32] * 6 + [C.POINTER(C.c_void_p)]),
+    "fg_rows_create": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int32, C.POINTER(FgTreeSeq), C.c_int32,
+                                 C.POINTER(C.c_void_p)]),
+    "fg_rows_set": (C.c_int, [C.c_void_p, C.POINTER(FgTreeSeq), C.c_int32]),
+    "fg_rows_destroy": (None, [C.c_void_p]),
+    "fg_rows_count": (C.c_int, [C.c_void_p, i32p, C.POINTER(C.c_int64), i32p]),
+    "fg_kv_append": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_int64]),
+    "fg_kv_gather": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p]),
+    "fg_kv_commit": (C.c_int, [C.c_void_p] * 5 + [C.c_int32]),
+    "fg_tree_attention": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_int64, C.c_void_p,
+                                    C.c_int64]),
+    "fg_tree_verify": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int32, C.c_int32] + [C.c_void_p] * 7 + [C.c_int32]),
+    "fg_tree_accept": (C.c_int, [C.c_void_p] * 7 + [C.c_int32]),
+    "fg_forward_tree": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.POINTER(FgTreeSeq), C.c_int32, f32p, u32p]),
+    "fg_tree_step": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.POINTER(FgTreeSeq), C.c_int32,
+                               C.POINTER(FgSampling), f32p, u32p, i32p, i32p, C.c_int32]),
     "fg_quantize": (C.c_int, [C.c_void_p, C.c_int32, C.c_int32, C.c_int32, f32p, f32p, u8p, f32p]),
     "fg_awq_search": (C.c_int, [C.c_void_p, C.c_int32, C.c_int32, C.c_int32, f32p, C.c_int32, f32p, f32p,
                                 C.POINTER(FgAwqChoice), u8p, f32p]),
@@ -219,9 +242,19 @@ class Context:
         h = C.c_void_p()
         check(lib().fg_ctx_create(device, C.byref(h)))
         self.h = h
+        self.device = device
 
     def sync(self) -> None:
         check(lib().fg_ctx_sync(self.h))
+
+    def wait(self, stream=0) -> None:
+        """What is queued on the context from now on runs after what `stream` (a hipStream_t as an int,
+        or an object with it as `cuda_stream`; 0: the default stream) holds now (fg_ctx_wait_stream)."""
+        check(lib().fg_ctx_wait_stream(self.h, getattr(stream, "cuda_stream", stream)))
+
+    def signal(self, stream=0) -> None:
+        """What is queued on `stream` from now on runs after what the context holds now (fg_stream_wait_ctx)."""
+        check(lib().fg_stream_wait_ctx(self.h, getattr(stream, "cuda_stream", stream)))
 
     def close(self) -> None:
         if getattr(self, "h", None):
@@ -292,16 +325,32 @@ class Model:
             self.close()
 
 
-class KvCache:
-    """Paged f32 KV cache on the device (fg_kv_create), reference layout."""
+KV_FORMATS = ("f32", "int8", "fp8")
 
-    def __init__(self, ctx: Context, cfg: Config, blocks: int, block_size: int = 16):
+
+@dataclass
+class CacheShape:
+    """What a KvCache needs to know of a model, where there is no Config of one."""
+    layers: int
+    kv_heads: int
+    head_dim: int
+
+
+class KvCache:
+    """Paged KV cache on the device (fg_kv_create_format): "f32" in the reference's layout, or keys and
+    values quantized to "int8" or "fp8" with a scale per token and head."""
+
+    def __init__(self, ctx: Context, cfg: Config | CacheShape, blocks: int, block_size: int = 16, format: str = "f32"):
+        if format not in KV_FORMATS:
+            raise ValueError(f"cache format {format!r}: one of {', '.join(KV_FORMATS)}")
         self.ctx = ctx
         self.cfg = cfg
         self.blocks = blocks
         self.block_size = block_size
+        self.format = format
         h = C.c_void_p()
-        check(lib().fg_kv_create(ctx.h, cfg.layers, cfg.kv_heads, cfg.head_dim, block_size, blocks, C.byref(h)))
+        check(lib().fg_kv_create_format(ctx.h, cfg.layers, cfg.kv_heads, cfg.head_dim, block_size, blocks,
+                                        KV_FORMATS.index(format), C.byref(h)))
         self.h = h
 
     def _n(self) -> int:
@@ -608,3 +657,199 @@ def awq_search(ctx: Context, kind: int, w: np.ndarray, cal: np.ndarray):
     check(lib().fg_awq_search(ctx.h, kind, rows, k, ptr(w, f32p), cal.shape[0], ptr(cal, f32p), ptr(sc, f32p),
                               C.byref(ch), ptr(q, u8p), ptr(s, f32p)))
     return sc, float(ch.alpha), float(ch.error_plain), float(ch.error_awq), Matrix(kind, rows, k, q=q, s=s)
+
+
+# ---------------------------------------------------------------------------
+# Rows over paged caches, on device arrays
+# ---------------------------------------------------------------------------
+@dataclass
+class TreeSeq:
+    """Rows of one sequence behind `pos` cached tokens (fg_tree_seq): a chain of n rows (parents an int), or a
+    tree (parents a list: an earlier row, -1 behind the cached tokens, -2 an unused row)."""
+    pos: int
+    blocks: np.ndarray | None
+    parents: int | list
+    tokens: np.ndarray | None = None
+
+
+def _tree_seqs(seqs: list, forward: bool = False):
+    """(the structs, the arrays that they point into)"""
+    arr = (FgTreeSeq * max(1, len(seqs)))()
+    keep = []
+    for i, s in enumerate(seqs):
+        chain = isinstance(s.parents, (int, np.integer))
+        par = None if chain else np.ascontiguousarray(s.parents, np.int32)
+        n = int(s.parents) if chain else len(par)
+        bl = None if s.blocks is None else np.ascontiguousarray(s.blocks, np.uint32)
+        tok = None
+        if forward:
+            if s.tokens is None or len(s.tokens) != n:
+                raise ValueError("one token per row")
+            tok = np.ascontiguousarray(s.tokens, np.uint32)
+        keep += [par, bl, tok]
+        arr[i] = FgTreeSeq(ptr(tok, u32p), n, s.pos, ptr(bl, u32p), 0 if bl is None else len(bl), 0, ptr(par, i32p))
+    return arr, keep
+
+
+class Rows:
+    """Rows of several sequences over caches of one shape, planned once for all layers of a step
+    (fg_rows_create): `total` rows, `tokens` cached tokens with the rows among them, `deepest` rows on the
+    longest branch. kv None: only the trees, for tree_verify and tree_accept. `set` plans the next step's
+    rows in the same handle."""
+
+    def __init__(self, ctx: Context, kv: KvCache | None, seqs: list, heads: int | None = None):
+        self.ctx = ctx
+        self.heads = heads if heads is not None else (kv.cfg.kv_heads if kv is not None else 1)
+        self.cfg = None if kv is None else kv.cfg
+        arr, keep = _tree_seqs(seqs)
+        h = C.c_void_p()
+        check(lib().fg_rows_create(ctx.h, None if kv is None else kv.h, self.heads, arr, len(seqs), C.byref(h)))
+        self.h = h
+        self._count(len(seqs))
+
+    def set(self, seqs: list) -> None:
+        arr, keep = _tree_seqs(seqs)
+        check(lib().fg_rows_set(self.h, arr, len(seqs)))
+        self._count(len(seqs))
+
+    def _count(self, seqs: int) -> None:
+        r, t, d = C.c_int32(), C.c_int64(), C.c_int32()
+        check(lib().fg_rows_count(self.h, C.byref(r), C.byref(t), C.byref(d)))
+        self.seqs, self.total, self.tokens, self.deepest = seqs, r.value, t.value, d.value
+
+    def close(self) -> None:
+        if getattr(self, "h", None):
+            lib().fg_rows_destroy(self.h)
+            self.h = None
+
+    def __del__(self):
+        if lib is not None:  # at interpreter exit the module's globals are already cleared
+            self.close()
+
+
+def _device(ctx: Context, a, what: str, dtype: str, shape: tuple, ld: bool = False):
+    """The address of a device array with torch's attributes (data_ptr, dtype, shape, stride, device), which
+    must have the type and shape; with ld also the distance of its rows, whose elements must be dense."""
+    if str(a.dtype) not in dtype or tuple(a.shape) != shape:
+        raise ValueError(f"{what}: expected {dtype} {list(shape)}, got {a.dtype} {list(a.shape)}")
+    if a.device.type != "cuda" or a.device.index != ctx.device:
+        raise ValueError(f"{what}: on {a.device}, the context is on GPU {ctx.device}")
+    if not ld:
+        if not a.is_contiguous():
+            raise ValueError(f"{what}: must be contiguous")
+        return a.data_ptr()
+    st = a.stride()
+    dense = 1
+    for n, d in zip(shape[:0:-1], st[:0:-1]):
+        if n > 1 and d != dense:
+            raise ValueError(f"{what}: each row must be dense")
+        dense *= n
+    return a.data_ptr(), (st[0] if shape[0] > 1 else dense)
+
+
+def _need_cache(rows: Rows, kv: KvCache) -> None:
+    if rows.cfg is None:
+        raise ValueError("these rows were planned without a cache")
+
+
+def kv_append(ctx: Context, rows: Rows, kv: KvCache, layer: int, k, v) -> None:
+    """Keys (already rotated) and values of the rows into the cache, quantized in its format (fg_kv_append):
+    float32 device arrays [rows][kv_heads][head_dim] with the same row stride."""
+    _need_cache(rows, kv)
+    shape = (rows.total, kv.cfg.kv_heads, kv.cfg.head_dim)
+    kp, ldk = _device(ctx, k, "k", "torch.float32", shape, ld=True)
+    vp, ldv = _device(ctx, v, "v", "torch.float32", shape, ld=True)
+    if ldk != ldv:
+        raise ValueError("k and v must have the same row stride")
+    check(lib().fg_kv_append(ctx.h, rows.h, kv.h, layer, kp, vp, ldk))
+
+
+def kv_gather(ctx: Context, rows: Rows, kv: KvCache, layer: int, k, v, context: bool = True) -> None:
+    """Cached keys and values back in float32 device arrays (fg_kv_gather): of every cached token of the
+    sequences [rows.tokens][kv_heads][head_dim], or of the rows [rows.total][...] (context False)."""
+    _need_cache(rows, kv)
+    shape = (rows.tokens if context else rows.total, kv.cfg.kv_heads, kv.cfg.head_dim)
+    check(lib().fg_kv_gather(ctx.h, rows.h, kv.h, layer, int(context), _device(ctx, k, "k", "torch.float32", shape),
+                             _device(ctx, v, "v", "torch.float32", shape)))
+
+
+def kv_commit(ctx: Context, rows: Rows, kv: KvCache, path, count) -> None:
+    """The accepted branches into place in every layer (fg_kv_commit): path int32 [seqs][ld] and count int32
+    [seqs], as tree_verify and tree_accept write them."""
+    _need_cache(rows, kv)
+    ld = path.shape[1]
+    check(lib().fg_kv_commit(ctx.h, rows.h, kv.h, _device(ctx, path, "path", "torch.int32", (rows.seqs, ld)),
+                             _device(ctx, count, "count", "torch.int32", (rows.seqs,)), ld))
+
+
+def tree_attention(ctx: Context, rows: Rows, kv: KvCache, layer: int, q, out) -> None:
+    """Attention of the rows over what they see of the cache (fg_tree_attention): float32 device arrays
+    [rows][heads][head_dim]."""
+    _need_cache(rows, kv)
+    shape = (rows.total, rows.heads, kv.cfg.head_dim)
+    qp, ldq = _device(ctx, q, "q", "torch.float32", shape, ld=True)
+    op, ldo = _device(ctx, out, "out", "torch.float32", shape, ld=True)
+    check(lib().fg_tree_attention(ctx.h, rows.h, kv.h, layer, qp, ldq, op, ldo))
+
+
+DRAFTS = ("each", "distinct", "fixed")
+
+
+def tree_verify(ctx: Context, rows: Rows, tokens, p, q, u, drafts: str, out_tokens, out_path, out_count) -> None:
+    """Verification of drafted trees from given uniform numbers (fg_tree_verify). Device arrays: tokens int32
+    or uint32 [rows], p and q float32 [rows][vocab] (q None when drafts is "fixed"), u float32 [rows], the
+    outputs int32 [seqs][ld], [seqs][ld] and [seqs]. drafts: "each" (siblings drawn independently),
+    "distinct" (without replacement) or "fixed" (given)."""
+    if drafts not in DRAFTS:
+        raise ValueError(f"drafts {drafts!r}: one of {', '.join(DRAFTS)}")
+    n, ld, vocab = rows.total, out_tokens.shape[1], p.shape[1]
+    ints = "torch.int32 torch.uint32"
+    check(lib().fg_tree_verify(
+        ctx.h, rows.h, DRAFTS.index(drafts), vocab, _device(ctx, tokens, "tokens", ints, (n,)),
+        _device(ctx, p, "p", "torch.float32", (n, vocab)),
+        None if q is None else _device(ctx, q, "q", "torch.float32", (n, vocab)),
+        _device(ctx, u, "u", "torch.float32", (n,)), _device(ctx, out_tokens, "out_tokens", ints, (rows.seqs, ld)),
+        _device(ctx, out_path, "out_path", "torch.int32", (rows.seqs, ld)),
+        _device(ctx, out_count, "out_count", "torch.int32", (rows.seqs,)), ld))
+
+
+def tree_accept(ctx: Context, rows: Rows, tokens, argmax, out_tokens, out_path, out_count) -> None:
+    """The greedy walk of drafted trees (fg_tree_accept): argmax int32 or uint32 [rows] is the target's token
+    behind each row; the rest as tree_verify."""
+    n, ld = rows.total, out_tokens.shape[1]
+    ints = "torch.int32 torch.uint32"
+    check(lib().fg_tree_accept(
+        ctx.h, rows.h, _device(ctx, tokens, "tokens", ints, (n,)), _device(ctx, argmax, "argmax", ints, (n,)),
+        _device(ctx, out_tokens, "out_tokens", ints, (rows.seqs, ld)),
+        _device(ctx, out_path, "out_path", "torch.int32", (rows.seqs, ld)),
+        _device(ctx, out_count, "out_count", "torch.int32", (rows.seqs,)), ld))
+
+
+def forward_tree(ctx: Context, model: Model, kv: KvCache, seqs: list, logits: bool = True) -> ForwardOut:
+    """Model::forward over trees of tokens with every row's logits and argmax (fg_forward_tree). seqs: TreeSeq
+    with tokens."""
+    arr, keep = _tree_seqs(seqs, forward=True)
+    n = sum(arr[i].n for i in range(len(seqs)))
+    lg = np.empty((n, model.cfg.vocab), np.float32) if logits else None
+    am = np.zeros(n, np.uint32)
+    check(lib().fg_forward_tree(ctx.h, model.h, kv.h, arr, len(seqs), ptr(lg, f32p), ptr(am, u32p)))
+    return ForwardOut(lg, am, None)
+
+
+def tree_step(ctx: Context, model: Model, kv: KvCache, seqs: list, params: list | None = None,
+              u: np.ndarray | None = None):
+    """One speculative step over given drafted trees (fg_tree_step): the target's forward, the walk (greedy,
+    or under per-sequence params with one uniform number per row), and the accepted branch's keys and values
+    into place. Returns (emitted tokens per sequence, the rows of each accepted branch)."""
+    arr, keep = _tree_seqs(seqs, forward=True)
+    n, rows = len(seqs), sum(arr[i].n for i in range(len(seqs)))
+    ld = max(1, max((arr[i].n for i in range(n)), default=1))
+    tok, path, cnt = np.zeros((n, ld), np.uint32), np.zeros((n, ld), np.int32), np.zeros(n, np.int32)
+    pr = None
+    if params is not None:
+        if len(params) != n or u is None or u.dtype != np.float32 or u.shape != (rows,) or not u.flags.c_contiguous:
+            raise ValueError("one parameter set per sequence and one float32 uniform number per row")
+        pr = _sampling_arrays(params)
+    check(lib().fg_tree_step(ctx.h, model.h, kv.h, arr, n, pr, ptr(u if pr is not None else None, f32p),
+                             ptr(tok, u32p), ptr(path, i32p), ptr(cnt, i32p), ld))
+    return [tok[i, :cnt[i]].copy() for i in range(n)], [path[i, :cnt[i]].copy() for i in range(n)]

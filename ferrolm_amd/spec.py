@@ -285,3 +285,113 @@ def generate(ctx: gpu.Context, target: gpu.Model, draft: gpu.Model | None, promp
     if stats is not None:
         stats.__dict__.update(r.stats.__dict__)
     return np.array(r.generated[:max_tokens], np.uint32)
+
+
+class TreeRunner:
+    """One request through tree speculation (ignore_eos): every step the draft model proposes a tree, level by
+    level the likeliest `fans[level]` tokens behind each node, and one target pass verifies it
+    (gpu.tree_step): greedily, or under params by the target's own distribution, with uniform numbers from
+    the request's seed. Caches may be of any format (tkv, dkv, or kv_format for both)."""
+
+    def __init__(self, ctx: gpu.Context, target: gpu.Model, draft: gpu.Model, prompt, fans=(4, 2, 1),
+                 kv_blocks: int = 1024, max_batch_tokens: int = 512, kv_format: str = "f32", tkv=None, dkv=None,
+                 params: gpu.SamplingParams | None = None):
+        self.ctx, self.target, self.draft, self.fans = ctx, target, draft, tuple(fans)
+        self.params = params if params is not None and not params.greedy else None
+        self.rng = np.array([gpu.rng_init(params.seed)], np.uint64) if self.params is not None else None
+        self.uniform = np.random.default_rng(params.seed) if self.params is not None else None
+        self.budget = max_batch_tokens
+        self.max_len = min(target.cfg.max_position, draft.cfg.max_position, kv_blocks * 16)
+        self.tokens = [int(t) for t in prompt]
+        if not self.tokens or len(self.tokens) >= self.max_len:
+            raise ValueError(f"prompt of {len(self.tokens)} tokens; this server fits 1 to {self.max_len - 1}")
+        self.tkv = tkv or gpu.KvCache(ctx, target.cfg, kv_blocks, format=kv_format)
+        self.dkv = dkv or gpu.KvCache(ctx, draft.cfg, kv_blocks, format=kv_format)
+        self.tpool, self.dpool = BlockPool(kv_blocks), BlockPool(kv_blocks)
+        self.tb, self.db = [], []
+        self.computed = self.dcomp = 0
+        self.generated = []
+        self.stats = GenStats()
+
+    def prefill(self) -> int:
+        """The first token, from the prompt in chunks of the token budget."""
+        n = len(self.tokens)
+        if not self.tpool.grow(self.tb, n):
+            raise RuntimeError("out of cache blocks")
+        while self.computed < n:
+            m = min(self.budget, n - self.computed)
+            last = self.computed + m == n
+            chunk = (self.tokens[self.computed:self.computed + m], self.computed, self.tb,
+                     gpu.LOGITS_LAST if last else gpu.LOGITS_NONE)
+            if last and self.params is not None:
+                first = int(gpu.forward_sampled(self.ctx, self.target, self.tkv, [chunk], [self.params], self.rng)[0])
+            else:
+                o = gpu.forward(self.ctx, self.target, self.tkv, [chunk], logits=False)
+                first = int(o.argmax[0]) if last else -1
+            self.computed += m
+        self.tokens.append(first)
+        self.generated.append(first)
+        return first
+
+    def propose(self):
+        """The draft's tree behind the last token: (tokens, parents) of its rows, the last token first."""
+        t, n = self.tokens, len(self.tokens)
+        tail = t[self.dcomp:]
+        while tail:  # the tokens that the draft has not seen
+            m = min(self.budget, len(tail))
+            o = gpu.forward(self.ctx, self.draft, self.dkv, [(tail[:m], self.dcomp, self.db,
+                                                              gpu.LOGITS_LAST if m == len(tail) else gpu.LOGITS_NONE)])
+            self.dcomp += m
+            tail = tail[m:]
+        tokens, parents, level, logits = [t[-1]], [-1], [0], o.logits
+        for depth, fan in enumerate(self.fans):
+            first = len(tokens)
+            for node, row in zip(level, logits):
+                best = np.argpartition(-row, fan - 1)[:fan]
+                for tok in best[np.lexsort((best, -row[best]))]:
+                    tokens.append(int(tok))
+                    parents.append(node)
+            level = list(range(first, len(tokens)))
+            if depth + 1 < len(self.fans):
+                # the whole tree again, behind the tokens that are settled: its last level is new
+                o = gpu.forward_tree(self.ctx, self.draft, self.dkv,
+                                     [gpu.TreeSeq(n, self.db, [p - 1 for p in parents[1:]], tokens[1:])])
+                logits = o.logits[first - 1:]
+        return tokens, parents
+
+    def step(self) -> list:
+        """One tree step; the emitted ids."""
+        n = len(self.tokens)
+        rows = 1
+        for fan in reversed(self.fans):
+            rows = 1 + fan * rows
+        if n + rows > self.max_len or not self.dpool.grow(self.db, n + rows):
+            tokens, parents = [self.tokens[-1]], [-1]  # no room for a tree: a plain step
+        else:
+            tokens, parents = self.propose()
+        if not self.tpool.grow(self.tb, n - 1 + len(tokens)):
+            raise RuntimeError("out of cache blocks")
+        u = None if self.params is None else self.uniform.random(len(tokens), np.float32)
+        out, _ = gpu.tree_step(self.ctx, self.target, self.tkv, [gpu.TreeSeq(n - 1, self.tb, parents, tokens)],
+                               None if self.params is None else [self.params], u)
+        emitted = [int(x) for x in out[0]][:self.max_len - n]
+        self.stats.spec_steps += 1
+        self.stats.proposed += len(tokens) - 1
+        self.stats.accepted += len(out[0]) - 1
+        self.stats.accepted_per_step.append(len(out[0]) - 1)
+        self.computed += len(out[0])
+        self.tokens += emitted
+        self.generated += emitted
+        return emitted
+
+
+def generate_tree(ctx: gpu.Context, target: gpu.Model, draft: gpu.Model, prompt, max_tokens: int, fans=(4, 2, 1),
+                  stats: GenStats | None = None, **kw):
+    """generate() by tree speculation (TreeRunner)."""
+    r = TreeRunner(ctx, target, draft, prompt, fans, **kw)
+    r.prefill()
+    while len(r.generated) < max_tokens and len(r.tokens) < r.max_len:
+        r.step()
+    if stats is not None:
+        stats.__dict__.update(r.stats.__dict__)
+    return np.array(r.generated[:max_tokens], np.uint32)

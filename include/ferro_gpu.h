@@ -38,11 +38,14 @@ extern "C" {
 
 enum { FG_BF16 = 0, FG_INT8 = 1, FG_INT4 = 2 };
 enum { FG_LOGITS_NONE = 0, FG_LOGITS_LAST = 1, FG_LOGITS_ALL = 2 }; /* src/model.rs:74-79 */
+enum { FG_KV_F32 = 0, FG_KV_INT8 = 1, FG_KV_FP8 = 2 };       /* cache formats (fg_kv_create_format) */
+enum { FG_DRAFT_EACH = 0, FG_DRAFT_DISTINCT = 1, FG_DRAFT_FIXED = 2 }; /* how siblings were drafted (fg_tree_verify) */
 
 typedef struct fg_ctx fg_ctx;
 typedef struct fg_model fg_model;
 typedef struct fg_kv fg_kv;
 typedef struct fg_mat fg_mat;
+typedef struct fg_rows fg_rows;
 
 /* Model hyperparameters: the fields of Config (src/config.rs:21-39) the
  * forward pass reads. */
@@ -106,6 +109,24 @@ typedef struct {
     int32_t n_draft_blocks;
 } fg_spec_seq;
 
+/* Rows of one sequence: `n` tokens in cache slots pos..pos+n-1, behind `pos`
+ * cached ones. parents NULL: a chain, every row sees the rows before it.
+ * Otherwise a tree of drafted tokens: parents[i] is an earlier row, whose
+ * branch row i continues, -1 (the row stands right behind the cached tokens)
+ * or -2 (the row is unused: nothing is written for it, and what is read for
+ * it is zeros). A row sees the cached tokens and its own branch, itself
+ * included; its position is pos + the number of rows before it on the branch.
+ * At most 4096 rows when not a chain. No reference counterpart: the
+ * reference drafts chains (src/engine.rs:658-717). */
+typedef struct {
+    const uint32_t* tokens; /* the forwards' (may be NULL elsewhere) */
+    int32_t n, pos;
+    const uint32_t* blocks; /* >= pos + n slots */
+    int32_t n_blocks;
+    int32_t _pad;
+    const int32_t* parents;
+} fg_tree_seq;
+
 /* The sampling fields of SamplingParams (src/sampler.rs:8-19, :34-38):
  * temperature <= 0 is greedy; otherwise logits are divided by
  * max(temperature, 1e-5), cut to the top_k largest (0: no limit, the whole
@@ -126,6 +147,14 @@ void fg_ctx_destroy(fg_ctx* ctx);
 const char* fg_last_error(void);
 /* Blocks until all work queued on the context has finished. */
 int fg_ctx_sync(fg_ctx* ctx);
+/* Order between the context and another HIP stream of its device (a
+ * hipStream_t; NULL is the default stream): what is queued on the context
+ * from now on runs after what `stream` holds now, and the other way round.
+ * Calls on device buffers that another stream fills or reads need the pair
+ * around them. While `stream` is captured into a graph, the calls between
+ * the pair are captured with it. */
+int fg_ctx_wait_stream(fg_ctx* ctx, void* stream);
+int fg_stream_wait_ctx(fg_ctx* ctx, void* stream);
 
 /* ---- weights ---------------------------------------------------------- */
 /* The shape checks of Config::parse (src/config.rs:70-74: heads divisible by
@@ -160,8 +189,20 @@ int fg_kv_create(fg_ctx* ctx, int32_t layers, int32_t kv_heads,
                  int32_t head_dim, int32_t block_size, int32_t blocks,
                  fg_kv** out);
 void fg_kv_destroy(fg_kv* kv);
+/* fg_kv_create with the keys and values held in `format`. FG_KV_INT8 and
+ * FG_KV_FP8 (OCP e4m3) keep, per token, head and K or V, head_dim codes of 8
+ * bits and an f32 scale: s = max|x| / 127 or / 448, codes x / s rounded to
+ * nearest (ties to even), each standing for code * s; both divisions are f32
+ * divisions, so the codes are defined bit for bit. A row of zeros has codes
+ * 0; one that holds an infinity or NaN stands for NaN throughout. The cache
+ * takes 2 * (head_dim + 4) bytes per token and head, 8 * head_dim in f32.
+ * Every call that takes an fg_kv takes all formats. */
+int fg_kv_create_format(fg_ctx* ctx, int32_t layers, int32_t kv_heads,
+                        int32_t head_dim, int32_t block_size, int32_t blocks,
+                        int32_t format, fg_kv** out);
 /* KvCache::layer (src/kv.rs:58-61): copies one layer's K and V to host
- * (each blocks*block_size*kv_heads*head_dim floats). For tests. */
+ * (each blocks*block_size*kv_heads*head_dim floats, the values that 8-bit
+ * codes stand for). For tests. */
 int fg_kv_read(fg_ctx* ctx, const fg_kv* kv, int32_t layer, float* k_out,
                float* v_out);
 /* Overwrites one layer's K and V from host. For tests and baselines. */
@@ -321,6 +362,107 @@ int fg_mm_tile(int32_t use, int32_t kind, int32_t n, int32_t k, int32_t m,
  * stream without synchronising. */
 int fg_matmul_device_noalloc(fg_ctx* ctx, const fg_mat* w, const float* x_dev,
                              int32_t m, float* y_dev);
+
+/* ---- rows over paged caches, on device buffers -------------------------- */
+/* Plans rows of `n_seqs` sequences over caches of `kv`'s heads, head_dim and
+ * blocks, for `heads` query heads, to be used for every layer of a step; kv
+ * NULL plans only their trees (fg_tree_verify, fg_tree_accept; blocks are not
+ * read). The host arrays are copied. The handle is the context's, and holds
+ * the attention's workspace: its calls run in order on the context's stream,
+ * and graphs that captured them share it, so they must not overlap. */
+int fg_rows_create(fg_ctx* ctx, const fg_kv* kv, int32_t heads,
+                   const fg_tree_seq* seqs, int32_t n_seqs, fg_rows** out);
+/* Plans other rows in the same handle (the next step's); calls queued before
+ * keep theirs. Graphs that captured calls with the handle are void after it.
+ * Refused (FG_E_ARG) while the context's stream is captured. */
+int fg_rows_set(fg_rows* rows, const fg_tree_seq* seqs, int32_t n_seqs);
+void fg_rows_destroy(fg_rows* rows);
+/* Rows, cached tokens with the rows among them, and rows on the longest
+ * branch (each may be NULL). */
+int fg_rows_count(const fg_rows* rows, int32_t* n_rows, int64_t* n_tokens,
+                  int32_t* deepest);
+
+/* The calls below are queued on the context's stream without synchronising;
+ * their arrays are device memory. Rows are counted over all sequences in
+ * order. f32 rows must be 16-byte aligned, ld* floats apart (a multiple of 4,
+ * so columns of a q/k/v matrix do as they are). */
+
+/* KvCache::write (src/kv.rs:48-56) of the rows, quantized as the cache's
+ * format says: k_dev and v_dev [row][kv_head][head_dim], keys already
+ * rotated. Slots of other tokens are left as they are. */
+int fg_kv_append(fg_ctx* ctx, const fg_rows* rows, fg_kv* kv, int32_t layer,
+                 const float* k_dev, const float* v_dev, int64_t ld);
+/* Reads keys and values back in f32, [token][kv_head][head_dim], contiguous:
+ * context 0 the rows', otherwise every cached token's of each sequence, the
+ * rows among them (unused ones as their slots are). */
+int fg_kv_gather(fg_ctx* ctx, const fg_rows* rows, const fg_kv* kv,
+                 int32_t layer, int32_t context, float* k_dev, float* v_dev);
+/* The accepted branch into place, in every layer: row path[s * ld + j] of
+ * sequence s moves to position pos + j, for j < count[s]. A path is a branch
+ * from its first row on, as fg_tree_verify writes it; rows that are not behind
+ * their place stay. */
+int fg_kv_commit(fg_ctx* ctx, const fg_rows* rows, fg_kv* kv,
+                 const int32_t* path_dev, const int32_t* count_dev, int32_t ld);
+/* Attention of the rows (Model::attention, src/model.rs:395-432, over
+ * trees): out[row][head] = sum over the tokens t that the row sees of
+ * softmax_t(q . k_t / sqrt(head_dim)) v_t; q_dev and out_dev
+ * [row][head][head_dim]. Unused rows get zeros. Reads the rows' own keys and
+ * values from the cache: fg_kv_append comes first. out may be q. */
+int fg_tree_attention(fg_ctx* ctx, const fg_rows* rows, const fg_kv* kv,
+                      int32_t layer, const float* q_dev, int64_t ldq,
+                      float* out_dev, int64_t ldo);
+/* Verification of drafted trees from given random numbers. Every sequence's
+ * row 0 is the last settled token and the root of its other rows, the drafted
+ * tokens. p_dev [row][vocab] is the target's distribution behind each row,
+ * q_dev the draft's that the row's children were drawn from: independently
+ * (FG_DRAFT_EACH), without replacement (FG_DRAFT_DISTINCT: the k-th child from
+ * q without its earlier siblings, over what they leave of 1; a child that this
+ * q can't have drawn is passed over, and all are once it leaves less than
+ * 2^-20), or not drawn at all (FG_DRAFT_FIXED, q_dev NULL: the draft's
+ * likeliest tokens, say). From row 0 on, the children of a row are tried in
+ * order of their rows: with P = p at first, child c of token t passes when
+ * q(t) > 0 and u[c] q(t) < P(t) (q(t) = 1 when not drawn), and a rejection
+ * leaves max(0, P - q) / sum (P without t when not drawn). Where no
+ * child passes, or there is none, u[row 0] draws the last token from what is
+ * left: the first whose cumulative sum, in token order, exceeds u * sum (from p
+ * when nothing is left). u_dev [row] uniform in [0, 1). A chain drawn from q is the
+ * reference's rule (src/engine.rs:575-610). All sums are in 64 bits; a NaN or
+ * negative probability counts as 0.
+ * out_tokens[s * ld + j], j < out_count[s]: the accepted tokens, then the
+ * drawn one; out_path[s * ld + j]: the rows whose distributions they came
+ * from, 0 first, so row out_path[j] holds emitted token j - 1. Past the count
+ * they hold 0 and -1. ld >= the rows of the longest branch. */
+int fg_tree_verify(fg_ctx* ctx, const fg_rows* rows, int32_t drafts,
+                   int32_t vocab, const uint32_t* tokens_dev,
+                   const float* p_dev, const float* q_dev, const float* u_dev,
+                   uint32_t* out_tokens_dev, int32_t* out_path_dev,
+                   int32_t* out_count_dev, int32_t ld);
+/* The greedy walk: argmax_dev [row] is the target's token behind each row;
+ * the first child that is its parent's passes. Outputs as fg_tree_verify. */
+int fg_tree_accept(fg_ctx* ctx, const fg_rows* rows,
+                   const uint32_t* tokens_dev, const uint32_t* argmax_dev,
+                   uint32_t* out_tokens_dev, int32_t* out_path_dev,
+                   int32_t* out_count_dev, int32_t ld);
+
+/* ---- forwards over trees ------------------------------------------------ */
+/* fg_forward over trees (or chains) of tokens, with every row's logits:
+ * logits_out (rows x vocab) and argmax_out (rows), host arrays, may be NULL.
+ * Unused rows are refused. */
+int fg_forward_tree(fg_ctx* ctx, const fg_model* m, fg_kv* kv,
+                    const fg_tree_seq* seqs, int32_t n_seqs, float* logits_out,
+                    uint32_t* argmax_out);
+/* One speculative step over given drafted trees, on the device: the
+ * target's forward over their rows, the walk (fg_tree_accept, or with params
+ * fg_tree_verify of given drafts under each sequence's sampling: p the
+ * distribution of fg_spec_step_sampled, sequences with temperature <= 0
+ * greedy), and fg_kv_commit of the accepted branch. u (one per row, host; only
+ * with params) as fg_tree_verify. Outputs as fg_tree_verify, host arrays. The
+ * caller's next step has pos + count cached tokens. */
+int fg_tree_step(fg_ctx* ctx, const fg_model* m, fg_kv* kv,
+                 const fg_tree_seq* seqs, int32_t n_seqs,
+                 const fg_sampling* params, const float* u,
+                 uint32_t* out_tokens, int32_t* out_path, int32_t* out_count,
+                 int32_t ld);
 
 /* ---- load-time quantization on the device ------------------------------ */
 /* QMatrix::quantize (src/quant.rs:78-143) on the device, bit for bit the
