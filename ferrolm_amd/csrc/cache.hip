@@ -3,10 +3,10 @@
 // same calls.
 //
 // A row of one head (HD channels of a token's key or value) has the scale
-// s = max|x| / 127 (int8) or max|x| / 448 (fp8 e4m3, whose largest value that
-// is); its codes are x / s rounded to nearest, ties to even, and stand for
-// code * s: off by at most half a step, s / 2 for int8 and 2^-4 of the value
-// for normal fp8 codes. Both divisions are IEEE divisions, so the codes are
+// s = max|x| * r, r = 1/127 (int8) or 1/448 (fp8 e4m3, whose largest value that
+// is) as f32; its codes are x / s rounded to nearest, ties to even, and stand
+// for code * s: off by at most half a step, s / 2 for int8 and 2^-4 of the
+// value for normal fp8 codes. The division is an IEEE one, so the codes are
 // the same wherever these steps are taken. A row of zeros, or whose scale
 // underflows, has codes 0; a row that holds an infinity or a NaN has the scale
 // NaN and codes 0, so that it reaches only what reads this row.
@@ -59,7 +59,7 @@ __device__ __forceinline__ float row_scale(const float (&x)[4]) {
     }
     m = group_reduce<HD / 4, true>(m);
     if (m == INFINITY) return NAN;
-    return m / (FMT == KV_INT8 ? 127.0f : 448.0f);
+    return m * (FMT == KV_INT8 ? 1.0f / 127.0f : 1.0f / 448.0f);
 }
 __device__ __forceinline__ void get4(const float* p, float (&x)[4]) {
     const float4 v = *(const float4*)p;

@@ -15,10 +15,10 @@
 // waves meet.
 //
 // Precision: int8 and fp8 codes are exact in f16. Queries are scaled by a power
-// of two and split into two f16, to 2^-21 of each input and 2^-31 of the
+// of two and split into two f16, to 2^-23 of each input or 2^-31 of the
 // largest; probabilities times value scales likewise. f32 keys and values are
 // scaled by row and split the same way (the product of the two small parts,
-// 2^-22, is left out). Sums are f32.
+// at most 2^-22, is left out). Sums are f32.
 #include "devutil.h"
 
 namespace fg {
@@ -67,12 +67,11 @@ __device__ __forceinline__ f32x4 mfma(f16x8 a, f16x8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
-// x = hi + lo, rounded towards zero: to 2^-21 of x, or 2^-24 where that is more (f16's smallest step)
+// x = hi + lo to 2^-23 of x, or 2^-25 where that is more (half of f16's smallest step)
 __device__ __forceinline__ void split2(float x0, float x1, uint32_t& hi, uint32_t& lo) {
-    const auto h = __builtin_amdgcn_cvt_pkrtz(x0, x1);
+    const f16x2 h = __builtin_convertvector((f32x2){x0, x1}, f16x2);
     hi = __builtin_bit_cast(uint32_t, h);
-    const f16x2 f = __builtin_bit_cast(f16x2, hi);
-    lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x0 - (float)f[0], x1 - (float)f[1]));
+    lo = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){x0 - (float)h[0], x1 - (float)h[1]}, f16x2));
 }
 __device__ __forceinline__ void split8(const float (&x)[8], f16x8& hi, f16x8& lo) {
     u32x4 h, l;

@@ -191,9 +191,9 @@ int fg_kv_create(fg_ctx* ctx, int32_t layers, int32_t kv_heads,
 void fg_kv_destroy(fg_kv* kv);
 /* fg_kv_create with the keys and values held in `format`. FG_KV_INT8 and
  * FG_KV_FP8 (OCP e4m3) keep, per token, head and K or V, head_dim codes of 8
- * bits and an f32 scale: s = max|x| / 127 or / 448, codes x / s rounded to
- * nearest (ties to even), each standing for code * s; both divisions are f32
- * divisions, so the codes are defined bit for bit. A row of zeros has codes
+ * bits and an f32 scale: s = max|x| * r, r = 1/127 or 1/448 rounded to f32,
+ * codes x / s (an f32 division) rounded to nearest, ties to even, at most 127
+ * or 448, each standing for code * s: defined bit for bit. A row of zeros has codes
  * 0; one that holds an infinity or NaN stands for NaN throughout. The cache
  * takes 2 * (head_dim + 4) bytes per token and head, 8 * head_dim in f32.
  * Every call that takes an fg_kv takes all formats. */

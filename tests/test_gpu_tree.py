@@ -30,7 +30,7 @@ def quantized(x, fmt):
     if fmt == "f32":
         return x, np.ones(x.shape[:-1] + (1,), np.float32)
     with np.errstate(invalid="ignore", divide="ignore", over="ignore"):
-        s = np.abs(x).max(axis=-1, keepdims=True) / np.float32(127 if fmt == "int8" else 448)
+        s = np.abs(x).max(axis=-1, keepdims=True) * (np.float32(1) / np.float32(127 if fmt == "int8" else 448))
         s = np.where(np.isfinite(x).all(axis=-1, keepdims=True), s, np.float32(np.nan)).astype(np.float32)
         y = np.where(s > 0, x / s, np.float32(0)).astype(np.float32)
         if fmt == "int8":
