@@ -20,7 +20,7 @@ namespace {
 // dword of codes; amax is the row's largest |x|, infinite where a value is not finite.
 template <int FMT>
 __device__ __forceinline__ uint32_t codes4(const float (&x)[4], float s) {
-    if (!(s > 0.0f)) return 0;  // zeros, or a NaN scale
+    if (!(s > 0.0f)) return FMT == KV_INT8 ? 0x80808080u : 0u;  // zeros, or a NaN scale
     float y[4];
 #pragma unroll
     for (int e = 0; e < 4; e++) y[e] = x[e] / s;
@@ -28,7 +28,7 @@ __device__ __forceinline__ uint32_t codes4(const float (&x)[4], float s) {
         uint32_t c = 0;
 #pragma unroll
         for (int e = 0; e < 4; e++) c |= ((uint32_t)(int)rintf(fminf(fmaxf(y[e], -127.0f), 127.0f)) & 255u) << (8 * e);
-        return c;
+        return c ^ 0x80808080u;
     } else {
 #pragma unroll
         for (int e = 0; e < 4; e++) y[e] = fminf(fmaxf(y[e], -448.0f), 448.0f);
@@ -40,7 +40,7 @@ template <int FMT>
 __device__ __forceinline__ void values4(uint32_t c, float s, float (&x)[4]) {
     if constexpr (FMT == KV_INT8) {
 #pragma unroll
-        for (int e = 0; e < 4; e++) x[e] = (float)(int8_t)(c >> (8 * e)) * s;
+        for (int e = 0; e < 4; e++) x[e] = ((float)(c >> (8 * e) & 255u) - 128.0f) * s;
     } else {
         x[0] = __builtin_amdgcn_cvt_f32_fp8(c, 0) * s;
         x[1] = __builtin_amdgcn_cvt_f32_fp8(c, 1) * s;

@@ -356,7 +356,8 @@ int stamps_clear(hipStream_t st);
 // A block of an 8-bit cache holds, per head, 16 tokens of HD channels as
 //   K codes [16 tokens][HD], V codes [4 token groups][HD][4 tokens],
 //   16 K scales, 16 V scales (f32)
-// in 32 HD + 128 consecutive bytes: [layer][block][kv head][record]. A row's value is code * scale. The
+// in 32 HD + 128 consecutive bytes: [layer][block][kv head][record]. A row's value is code * scale; int8
+// codes are held plus 128, from where a byte becomes an f16 with one operation fewer. The
 // layouts are those of the MFMA operands (k_tree_attn): a lane's keys are HD / 4 consecutive bytes, its
 // values HD / 4 too, and what a wave reads of a record is contiguous.
 // ---------------------------------------------------------------------------

@@ -3,7 +3,11 @@
 //
 // Row i of a sequence with `pos` cached tokens before its rows attends to
 // those and to its own branch: o = sum_t softmax_t(q . k_t / sqrt(HD)) v_t,
-// one pass with a running maximum m and sum l per query.
+// one pass with a running reference m and sum l per query: a token's probability
+// is p = 2^(score - m), its weight w = p * (its value's scale), and the output
+// sum w code / sum p, from which m cancels. m rises only when a weight would
+// leave f16 (kMost) or a probability grow out of bounds, so most steps compare
+// and branch once where a running maximum would reduce across lanes.
 //
 // A wave holds up to 16 QT queries (rows x grouped heads, a slot) of one kv
 // head and takes pairs of pages. Both products run transposed on f16 MFMA
@@ -32,6 +36,9 @@ namespace {
 constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
 // Below every score; its exponential is 0 against any.
 constexpr float kLowest = -1e30f;
+// A weight past kMost, or a probability past kMostP (its value may be zero), raises the reference to where the
+// largest weight is 2^kTop and no probability above 2^kTopP.
+constexpr float kMost = 32768.0f, kMostP = 0x1p60f, kTop = 9.0f, kTopP = 40.0f;
 
 // Eight codes, of which d0 holds the first four, in f16.
 template <int FMT>
@@ -39,11 +46,10 @@ __device__ __forceinline__ f16x8 codes8(uint32_t d0, uint32_t d1) {
     uint32_t h[4];
     if constexpr (FMT == KV_INT8) {
         // 0x6400 | (code + 128) is 1152 + code as f16
-        const uint32_t x0 = d0 ^ 0x80808080u, x1 = d1 ^ 0x80808080u;
-        h[0] = __builtin_amdgcn_perm(0x64646464u, x0, 0x04010400u);
-        h[1] = __builtin_amdgcn_perm(0x64646464u, x0, 0x04030402u);
-        h[2] = __builtin_amdgcn_perm(0x64646464u, x1, 0x04010400u);
-        h[3] = __builtin_amdgcn_perm(0x64646464u, x1, 0x04030402u);
+        h[0] = __builtin_amdgcn_perm(0x64646464u, d0, 0x04010400u);
+        h[1] = __builtin_amdgcn_perm(0x64646464u, d0, 0x04030402u);
+        h[2] = __builtin_amdgcn_perm(0x64646464u, d1, 0x04010400u);
+        h[3] = __builtin_amdgcn_perm(0x64646464u, d1, 0x04030402u);
         f16x8 r;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
@@ -69,9 +75,11 @@ __device__ __forceinline__ f32x4 mfma(f16x8 a, f16x8 b, f32x4 c) {
 
 // x = hi + lo to 2^-23 of x, or 2^-25 where that is more (half of f16's smallest step)
 __device__ __forceinline__ void split2(float x0, float x1, uint32_t& hi, uint32_t& lo) {
-    const f16x2 h = __builtin_convertvector((f32x2){x0, x1}, f16x2);
-    hi = __builtin_bit_cast(uint32_t, h);
-    lo = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){x0 - (float)h[0], x1 - (float)h[1]}, f16x2));
+    hi = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){x0, x1}, f16x2));
+    float y0, y1;  // x - hi, the f16 operand widened by the operation itself
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(y0) : "v"(hi), "v"(x0));
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(y1) : "v"(hi), "v"(x1));
+    lo = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){y0, y1}, f16x2));
 }
 __device__ __forceinline__ void split8(const float (&x)[8], f16x8& hi, f16x8& lo) {
     u32x4 h, l;
@@ -93,15 +101,14 @@ __device__ __forceinline__ int split_exp(float m) {
     return max(e, -100) - 6;
 }
 
-// What a lane takes of a page: keys of token lane % 16 at channels (lane / 16) HD / 4 .., values of tokens
-// 4 (lane / 16) .. +3 at channels (lane % 16) HD / 16 .., and the scales of those four tokens.
+// What a lane takes of a page: the key of token lane % 16 at channels (lane / 16) HD / 4 .., and the values of
+// tokens 4 (lane / 16) .. +3 at channels (lane % 16) HD / 16 .., each with the scales of those four tokens.
 template <int HD, int FMT>
-struct Page {
+struct Half {  // 8-bit formats: the codes
     static constexpr int KD = HD / 16;
-    uint32_t k[KD], v[KD];
-    float4 ks, vs;
-    template <class T>
-    static __device__ __forceinline__ void words(const uint8_t* p, T* d) {
+    uint32_t d[KD];
+    float4 s;
+    __device__ __forceinline__ void load(const uint8_t* p, const uint8_t* scales) {
         if constexpr (KD == 1) {
             d[0] = *(const uint32_t*)p;
         } else if constexpr (KD == 2) {
@@ -115,105 +122,114 @@ struct Page {
                 for (int e = 0; e < 4; e++) d[4 * i + e] = x[e];
             }
         }
+        s = *(const float4*)scales;
     }
+};
+template <int HD, int FMT>
+struct KeyPage : Half<HD, FMT> {
     __device__ __forceinline__ void load(const KvLayer& kv, size_t block, int h, int lane) {
         const uint8_t* rec = kv.data + (block * kv.nkv + h) * kv_record(HD);
-        const int r = lane & 15, g = lane >> 4;
-        words(rec + r * HD + g * (HD / 4), k);
-        words(rec + 16 * HD + g * (4 * HD) + r * (HD / 4), v);
-        ks = *(const float4*)(rec + 32 * HD + 16 * g);
-        vs = *(const float4*)(rec + 32 * HD + 64 + 16 * g);
+        Half<HD, FMT>::load(rec + (lane & 15) * HD + (lane >> 4) * (HD / 4), rec + 32 * HD + (lane >> 4) * 16);
+    }
+};
+template <int HD, int FMT>
+struct ValuePage : Half<HD, FMT> {
+    __device__ __forceinline__ void load(const KvLayer& kv, size_t block, int h, int lane) {
+        const uint8_t* rec = kv.data + (block * kv.nkv + h) * kv_record(HD) + 16 * HD;
+        Half<HD, FMT>::load(rec + (lane >> 4) * (4 * HD) + (lane & 15) * (HD / 4), rec + 16 * HD + 64 + (lane >> 4) * 16);
     }
 };
 template <int HD>
-struct Page<HD, KV_F32> {
-    static constexpr int N = HD / 4, C = HD / 16;  // a lane's key channels; its value channels of each of four tokens
-    float k[N], v[4][C];
+struct KeyPage<HD, KV_F32> {
+    float d[HD / 4];
     __device__ __forceinline__ void load(const KvLayer& kv, size_t block, int h, int lane) {
-        const size_t at = (block * kv.nkv + h) * 16 * HD;
-        const int r = lane & 15, g = lane >> 4;
-        const float* kp = kv.k + at + r * HD + g * N;
+        const float* p = kv.k + (block * kv.nkv + h) * 16 * HD + (lane & 15) * HD + (lane >> 4) * (HD / 4);
 #pragma unroll
-        for (int i = 0; i < N; i += 4) {
-            const float4 x = *(const float4*)(kp + i);
-            k[i] = x.x, k[i + 1] = x.y, k[i + 2] = x.z, k[i + 3] = x.w;
+        for (int i = 0; i < HD / 4; i += 4) {
+            const float4 x = *(const float4*)(p + i);
+            d[i] = x.x, d[i + 1] = x.y, d[i + 2] = x.z, d[i + 3] = x.w;
         }
+    }
+};
+template <int HD>
+struct ValuePage<HD, KV_F32> {
+    static constexpr int C = HD / 16;  // channels of each of the four tokens
+    float d[4][C];
+    __device__ __forceinline__ void load(const KvLayer& kv, size_t block, int h, int lane) {
 #pragma unroll
         for (int t = 0; t < 4; t++) {
-            const float* vp = kv.v + at + (4 * g + t) * HD + r * C;
+            const float* p = kv.v + ((block * kv.nkv + h) * 16 + 4 * (lane >> 4) + t) * HD + (lane & 15) * C;
             if constexpr (C >= 4) {
 #pragma unroll
                 for (int i = 0; i < C; i += 4) {
-                    const float4 x = *(const float4*)(vp + i);
-                    v[t][i] = x.x, v[t][i + 1] = x.y, v[t][i + 2] = x.z, v[t][i + 3] = x.w;
+                    const float4 x = *(const float4*)(p + i);
+                    d[t][i] = x.x, d[t][i + 1] = x.y, d[t][i + 2] = x.z, d[t][i + 3] = x.w;
                 }
             } else if constexpr (C == 2) {
-                const float2 x = *(const float2*)vp;
-                v[t][0] = x.x, v[t][1] = x.y;
+                const float2 x = *(const float2*)p;
+                d[t][0] = x.x, d[t][1] = x.y;
             } else {
-                v[t][0] = *vp;
+                d[t][0] = *p;
             }
         }
     }
 };
 
-// A page as MFMA operands: the scores' key operand by steps of 32 channels, and the scales of the lane's four
-// tokens. lo is there for f32 caches only.
+// A page's keys as MFMA operands, by steps of 32 channels (lo for f32 caches only), and the scales of the lane's
+// four tokens.
 template <int HD, int FMT>
 struct Keys {
     static constexpr int NS = HD >= 32 ? HD / 32 : 1;
     f16x8 hi[NS], lo[FMT == KV_F32 ? NS : 1];
     float s[4];
+    __device__ __forceinline__ explicit Keys(const KeyPage<HD, FMT>& p, int lane) {
+        if constexpr (FMT == KV_F32) {
+            float m = 0.0f;
+#pragma unroll
+            for (int i = 0; i < HD / 4; i++) m = fmaxf(m, fabsf(p.d[i]) <= 3.4e38f ? fabsf(p.d[i]) : INFINITY);
+            m = reduce_rows<true, true>(m);
+            const bool fine = m < INFINITY;
+            const int e = split_exp(m);
+            const float f = ldexpf(1.0f, -e);
+            const float sc = fine ? ldexpf(1.0f, e) : NAN;  // of key lane % 16
+#pragma unroll
+            for (int j = 0; j < NS; j++) {
+                float x[8];
+#pragma unroll
+                for (int i = 0; i < 8; i++) x[i] = 8 * j + i < HD / 4 && fine ? p.d[(8 * j + i) % (HD / 4)] * f : 0.0f;
+                split8(x, hi[j], lo[j]);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) s[i] = __shfl(sc, 4 * (lane >> 4) + i);
+        } else {
+#pragma unroll
+            for (int j = 0; j < NS; j++)
+                hi[j] = codes8<FMT>(p.d[(2 * j) % (HD / 16)], HD >= 32 ? p.d[(2 * j + 1) % (HD / 16)] : 0u);
+            if constexpr (HD == 16) {  // only four channels a lane: the operand's other half is zero
+#pragma unroll
+                for (int i = 4; i < 8; i++) hi[0][i] = (_Float16)0.0f;
+            }
+            s[0] = p.s.x, s[1] = p.s.y, s[2] = p.s.z, s[3] = p.s.w;
+        }
+    }
 };
 
+// Scales of the lane's four values of a page, and for f32 the factors to split them by (0: not finite).
 template <int HD, int FMT>
-__device__ __forceinline__ void make_keys(const Page<HD, FMT>& p, Keys<HD, FMT>& o, int lane) {
-    if constexpr (FMT == KV_F32) {
-        float m = 0.0f;
-#pragma unroll
-        for (int i = 0; i < HD / 4; i++) m = fmaxf(m, fabsf(p.k[i]) <= 3.4e38f ? fabsf(p.k[i]) : INFINITY);
-        m = reduce_rows<true, true>(m);
-        const bool fine = m < INFINITY;
-        const int e = split_exp(m);
-        const float f = ldexpf(1.0f, -e);
-        const float sc = fine ? ldexpf(1.0f, e) : NAN;  // of key lane % 16
-#pragma unroll
-        for (int s = 0; s < Keys<HD, FMT>::NS; s++) {
-            float x[8];
-#pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = 8 * s + i < HD / 4 && fine ? p.k[(8 * s + i) % (HD / 4)] * f : 0.0f;
-            split8(x, o.hi[s], o.lo[s]);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; i++) o.s[i] = __shfl(sc, 4 * (lane >> 4) + i);
-    } else {
-#pragma unroll
-        for (int s = 0; s < Keys<HD, FMT>::NS; s++)
-            o.hi[s] = codes8<FMT>(p.k[(2 * s) % (HD / 16)], HD >= 32 ? p.k[(2 * s + 1) % (HD / 16)] : 0u);
-        if constexpr (HD == 16) {  // only four channels a lane: the operand's other half is zero
-#pragma unroll
-            for (int i = 4; i < 8; i++) o.hi[0][i] = (_Float16)0.0f;
-        }
-        o.s[0] = p.ks.x, o.s[1] = p.ks.y, o.s[2] = p.ks.z, o.s[3] = p.ks.w;
-    }
-}
-
-// Scales of the lane's four values of a page, and for f32 the exponent to split them by.
-template <int HD, int FMT>
-__device__ __forceinline__ void value_scales(const Page<HD, FMT>& p, float (&s)[4], float (&f)[4]) {
+__device__ __forceinline__ void value_scales(const ValuePage<HD, FMT>& p, float (&s)[4], float (&f)[4]) {
     if constexpr (FMT == KV_F32) {
 #pragma unroll
         for (int t = 0; t < 4; t++) {
             float m = 0.0f;
 #pragma unroll
-            for (int i = 0; i < HD / 16; i++) m = fmaxf(m, fabsf(p.v[t][i]) <= 3.4e38f ? fabsf(p.v[t][i]) : INFINITY);
+            for (int i = 0; i < HD / 16; i++) m = fmaxf(m, fabsf(p.d[t][i]) <= 3.4e38f ? fabsf(p.d[t][i]) : INFINITY);
             m = group_reduce<16, true>(m);
             const int e = split_exp(m);
             s[t] = m < INFINITY ? ldexpf(1.0f, e) : NAN;
             f[t] = m < INFINITY ? ldexpf(1.0f, -e) : 0.0f;
         }
     } else {
-        s[0] = p.vs.x, s[1] = p.vs.y, s[2] = p.vs.z, s[3] = p.vs.w;
+        s[0] = p.s.x, s[1] = p.s.y, s[2] = p.s.z, s[3] = p.s.w;
     }
 }
 
@@ -226,7 +242,7 @@ __global__ __launch_bounds__(512) void k_tree_attn(RowArgs a, KvLayer kv, TreeAt
     constexpr int KD = HD / 16, NS = Keys<HD, FMT>::NS;
     constexpr int QM = HD >= 64 ? 32 : 64;
     constexpr bool F32 = FMT == KV_F32;
-    constexpr int ND = 4 * KD + 3;  // dwords a lane keeps of a tile
+    constexpr int ND = 4 * KD + 2;  // dwords a lane keeps of a tile
     extern __shared__ float sh[];
     const int h = blockIdx.x % kv.nkv, item = blockIdx.x / kv.nkv;
     const int4 i0 = *(const int4*)(a.items + (size_t)item * kItemWords),
@@ -242,17 +258,13 @@ __global__ __launch_bounds__(512) void k_tree_attn(RowArgs a, KvLayer kv, TreeAt
     const bool on = slot < i1.z && nr > 0;
 
     f16x8 qh[QT][NS], ql[QT][NS];
-    // score factor; running maximum (log 2 units) and sum; the power of two at or above the value scales so far (a
-    // weight is the probability times the value scale over it, in [0, 1], times 2^13 for the split), 2^13 over it
-    float qf[QT], mq[QT], l[QT], ec[QT], vn[QT];
+    float qf[QT], mq[QT], l[QT];  // score factor (log 2 units), reference, sum of probabilities
     int qrow[QT];                          // the query's row in its sequence
     f32x4 o[QT][KD];
 #pragma unroll
     for (int i = 0; i < QT; i++) {
         mq[i] = kLowest;
         l[i] = 0.0f;
-        ec[i] = 0x1p-100f;
-        vn[i] = 0x1p113f;
         qf[i] = 1.0f;
         qrow[i] = 0;
 #pragma unroll
@@ -303,18 +315,22 @@ __global__ __launch_bounds__(512) void k_tree_attn(RowArgs a, KvLayer kv, TreeAt
             const int pg = i0.z + 2 * (share + a.pw * (c0 + lane / 2)) + (lane & 1);
             const int ids = a.btab[btab + min(pg, last - 1)];
             const int np = min(32, mine - c0);
+            // keys and values are asked for as soon as the registers of the pair before are free: the keys behind
+            // the scores, the values behind the weighted sum
+            KeyPage<HD, FMT> kp[2];
+            ValuePage<HD, FMT> vp[2];
+            auto block = [&](int c, int x) { return (size_t)(uint32_t)__builtin_amdgcn_readlane(ids, 2 * c + x); };
+#pragma unroll
+            for (int x = 0; x < 2; x++) kp[x].load(kv, block(0, x), h, lane);
+#pragma unroll
+            for (int x = 0; x < 2; x++) vp[x].load(kv, block(0, x), h, lane);
             for (int c = 0; c < np; c++) {
                 const int p0 = i0.z + 2 * (share + a.pw * (c0 + c));  // the pair's first page
-                Page<HD, FMT> pg2[2];
-#pragma unroll
-                for (int x = 0; x < 2; x++)
-                    pg2[x].load(kv, (size_t)(uint32_t)__builtin_amdgcn_readlane(ids, 2 * c + x), h, lane);
-                float raw[2][QT][4], vsc[2][4], vf[2][4];
+                const int next = min(c + 1, np - 1);
+                float raw[2][QT][4];
 #pragma unroll
                 for (int x = 0; x < 2; x++) {
-                    Keys<HD, FMT> k;
-                    make_keys<HD, FMT>(pg2[x], k, lane);
-                    value_scales<HD, FMT>(pg2[x], vsc[x], vf[x]);
+                    const Keys<HD, FMT> k(kp[x], lane);
 #pragma unroll
                     for (int i = 0; i < QT; i++) {
                         f32x4 acc = (f32x4){0, 0, 0, 0};
@@ -328,9 +344,9 @@ __global__ __launch_bounds__(512) void k_tree_attn(RowArgs a, KvLayer kv, TreeAt
                         for (int e = 0; e < 4; e++) raw[x][i][e] = acc[e] * k.s[e];
                     }
                 }
-                const bool masked = 16 * (p0 + 2) > full || p0 + 1 >= last;
-                float vmax = 0.0f;
-                if (masked) {
+#pragma unroll
+                for (int x = 0; x < 2; x++) kp[x].load(kv, block(next, x), h, lane);
+                if (16 * (p0 + 2) > full || p0 + 1 >= last) {
 #pragma unroll
                     for (int x = 0; x < 2; x++)
 #pragma unroll
@@ -344,47 +360,53 @@ __global__ __launch_bounds__(512) void k_tree_attn(RowArgs a, KvLayer kv, TreeAt
 #pragma unroll
                             for (int e = 0; e < 4; e++) raw[x][i][e] = sees >> e & 1 ? raw[x][i][e] : -INFINITY;
                         }
-                } else {
-#pragma unroll
-                    for (int x = 0; x < 2; x++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++) vmax = fmaxf(vmax, vsc[x][e]);
-                    vmax = reduce_rows<true, true>(vmax);
                 }
+                float vsc[2][4], vf[2][4];
+#pragma unroll
+                for (int x = 0; x < 2; x++) value_scales<HD, FMT>(vp[x], vsc[x], vf[x]);
                 uint32_t ph[QT][4], pl[QT][4];
 #pragma unroll
                 for (int i = 0; i < QT; i++) {
-                    float mx = -INFINITY, vm = vmax;
+                    float p[8], w[8];
+                    auto weigh = [&] {
 #pragma unroll
-                    for (int x = 0; x < 2; x++)
+                        for (int x = 0; x < 2; x++)
 #pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            mx = fmaxf(mx, raw[x][i][e]);
-                            if (masked && raw[x][i][e] != -INFINITY) vm = fmaxf(vm, vsc[x][e]);
-                        }
-                    mx = reduce_rows<true, true>(mx);
-                    if (masked) vm = reduce_rows<true, true>(vm);
-                    const float mn = fmaxf(mq[i], mx * qf[i]);
-                    // the power of two at or above the largest value scale
-                    const float en = fmaxf(ec[i], __uint_as_float((__float_as_uint(vm) + 0x7FFFFFu) & 0x7F800000u));
-                    if (__any(mn > mq[i] || en > ec[i])) {
-                        const float f = __builtin_amdgcn_exp2f(mq[i] - mn), fo = f * (ec[i] / en);
+                            for (int e = 0; e < 4; e++) {
+                                const float y = __builtin_amdgcn_exp2f(fmaf(raw[x][i][e], qf[i], -mq[i]));
+                                p[4 * x + e] = y;
+                                w[4 * x + e] = y * vsc[x][e];
+                            }
+                    };
+                    weigh();
+                    float wm = 0.0f, pm = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        wm = fmaxf(wm, w[e]);
+                        pm = fmaxf(pm, p[e]);
+                    }
+                    if (__any(wm > kMost || pm > kMostP)) {
+                        float top = -INFINITY;
+#pragma unroll
+                        for (int x = 0; x < 2; x++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) {
+                                const float sc = raw[x][i][e] * qf[i];
+                                top = fmaxf(top, fmaxf(sc + __builtin_amdgcn_logf(vsc[x][e]) - kTop, sc - kTopP));
+                            }
+                        const float mn = fmaxf(mq[i], reduce_rows<true, true>(top)), f = __builtin_amdgcn_exp2f(mq[i] - mn);
                         l[i] *= f;
 #pragma unroll
-                        for (int j = 0; j < KD; j++) o[i][j] *= fo;
+                        for (int j = 0; j < KD; j++) o[i][j] *= f;
                         mq[i] = mn;
-                        ec[i] = en;
-                        vn[i] = 8192.0f / en;
+                        weigh();
                     }
-                    float w[8];
+                    // a value that is not finite has a NaN scale, which must not reach the rows that don't see it
 #pragma unroll
-                    for (int x = 0; x < 2; x++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            const float p = __builtin_amdgcn_exp2f(fmaf(raw[x][i][e], qf[i], -mq[i]));
-                            l[i] += p;
-                            w[4 * x + e] = masked && raw[x][i][e] == -INFINITY ? 0.0f : p * (vsc[x][e] * vn[i]);
-                        }
+                    for (int e = 0; e < 8; e++) {
+                        l[i] += p[e];
+                        w[e] = p[e] == 0.0f ? 0.0f : w[e];
+                    }
 #pragma unroll
                     for (int e = 0; e < 4; e++) split2(w[2 * e], w[2 * e + 1], ph[i][e], pl[i][e]);
                 }
@@ -396,10 +418,10 @@ __global__ __launch_bounds__(512) void k_tree_attn(RowArgs a, KvLayer kv, TreeAt
 #pragma unroll
                         for (int x = 0; x < 2; x++)
 #pragma unroll
-                            for (int e = 0; e < 4; e++) y[4 * x + e] = vf[x][e] == 0.0f ? 0.0f : pg2[x].v[e][j] * vf[x][e];
+                            for (int e = 0; e < 4; e++) y[4 * x + e] = vf[x][e] == 0.0f ? 0.0f : vp[x].d[e][j] * vf[x][e];
                         split8(y, vh, vl);
                     } else {
-                        vh = codes8<FMT>(pg2[0].v[j], pg2[1].v[j]);
+                        vh = codes8<FMT>(vp[0].d[j], vp[1].d[j]);
                     }
 #pragma unroll
                     for (int i = 0; i < QT; i++) {
@@ -410,6 +432,8 @@ __global__ __launch_bounds__(512) void k_tree_attn(RowArgs a, KvLayer kv, TreeAt
                         o[i][j] = mfma(vh, hi, o[i][j]);
                     }
                 }
+#pragma unroll
+                for (int x = 0; x < 2; x++) vp[x].load(kv, block(next, x), h, lane);
             }
         }
 #pragma unroll
@@ -423,24 +447,21 @@ __global__ __launch_bounds__(512) void k_tree_attn(RowArgs a, KvLayer kv, TreeAt
             if (on && share >= half && share < 2 * half) {
                 x[0] = mq[i];
                 x[64] = l[i];
-                x[128] = ec[i];
 #pragma unroll
                 for (int j = 0; j < KD; j++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) x[(3 + 4 * j + e) * 64] = o[i][j][e];
+                    for (int e = 0; e < 4; e++) x[(2 + 4 * j + e) * 64] = o[i][j][e];
             }
             __syncthreads();
             if (on && share < half) {
-                const float m2 = x[0], mn = fmaxf(mq[i], m2), en = fmaxf(ec[i], x[128]);
+                const float m2 = x[0], mn = fmaxf(mq[i], m2);
                 const float f1 = __builtin_amdgcn_exp2f(mq[i] - mn), f2 = __builtin_amdgcn_exp2f(m2 - mn);
-                const float w1 = f1 * (ec[i] / en), w2 = f2 * (x[128] / en);
                 l[i] = l[i] * f1 + x[64] * f2;
 #pragma unroll
                 for (int j = 0; j < KD; j++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) o[i][j][e] = o[i][j][e] * w1 + x[(3 + 4 * j + e) * 64] * w2;
+                    for (int e = 0; e < 4; e++) o[i][j][e] = o[i][j][e] * f1 + x[(2 + 4 * j + e) * 64] * f2;
                 mq[i] = mn;
-                ec[i] = en;
             }
             __syncthreads();
         }
@@ -450,13 +471,12 @@ __global__ __launch_bounds__(512) void k_tree_attn(RowArgs a, KvLayer kv, TreeAt
     for (int i = 0; i < QT; i++) {
         const int qi = 16 * i + r;
         if (qi >= Q) continue;
-        const float sc = ec[i] * (1.0f / 8192.0f);
         float* dst;
-        float f = sc;
+        float f = 1.0f;
         if (t.out && i1.w) {
             // no other item has these rows: what they attend to, zeros where that is nothing
             const bool none = l[i] == 0.0f || a.mrec[(size_t)(seq0 + qrow[i]) * 4 + 3];
-            f = none ? 0.0f : sc / l[i];
+            f = none ? 0.0f : 1.0f / l[i];
             if (none) {
 #pragma unroll
                 for (int j = 0; j < KD; j++) o[i][j] = (f32x4){0, 0, 0, 0};
@@ -538,7 +558,7 @@ __global__ __launch_bounds__(256) void k_tree_merge(RowArgs a, TreeAttn t, int n
 template <int HD, int FMT>
 static void tree_qt(hipStream_t st, const RowArgs& a, const KvLayer& kv, const TreeAttn& t) {
     const dim3 grid((unsigned)kv.nkv * a.n_items), block(64 * a.rw * a.pw);
-    const size_t per = (size_t)64 * 4 * (4 * (HD / 16) + 3) * (a.pw / 2) * a.rw;
+    const size_t per = (size_t)64 * 4 * (4 * (HD / 16) + 2) * (a.pw / 2) * a.rw;
     constexpr int QT = HD >= 64 ? 2 : 4;
     if (a.qt == 1)
         hipLaunchKernelGGL((k_tree_attn<HD, FMT, 1>), grid, block, per, st, a, kv, t);
