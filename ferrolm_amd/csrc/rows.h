@@ -20,8 +20,9 @@ struct RowSeq {
 
 // Longest tree: its masks hold a bit per row and token of the tree.
 constexpr int kTreeRows = 4096;
-// Workgroups that an attention launch is cut into where the context allows.
-constexpr int kTreeTarget = 512;
+// Workgroups that an attention launch is cut into at most, where it has not more row groups: what the card
+// runs at a time, one workgroup a CU of several slots, two of one.
+constexpr int tree_workgroups(int rw) { return rw > 1 ? 256 : 512; }
 
 struct RowPlan {
     int n_seqs = 0, rows = 0, n_wi = 0, n_items = 0, n_quads = 0, longest = 0, deepest = 0, widest = 0;
@@ -126,18 +127,32 @@ inline void plan_rows(RowPlan& P, const RowSeq* in, int n_seqs, int nh, int nkv,
         const int last = chain ? q.pos + std::min(q.n, r0 + P.rw * rps) : q.pos + q.n;
         return (last + 15) / 16;
     };
-    int64_t work = 0;
+    // the shortest parts, in whole rounds of a workgroup's waves, that make no more workgroups than that
+    const int step = 2 * P.pw;
+    std::vector<int> groups;  // pages of every row group
     for (int s = 0; cached && s < n_seqs; s++)
-        for (int r0 = 0; r0 < in[s].n; r0 += P.rw * rps) work += group_pages(in[s], r0);
-    const int step = 2 * P.pw;  // pages of one round of the workgroup's waves
-    int64_t len = (work * nkv + kTreeTarget - 1) / kTreeTarget;
-    len = std::max<int64_t>((len + step - 1) / step * step, step);
+        for (int r0 = 0; r0 < in[s].n; r0 += P.rw * rps) groups.push_back(group_pages(in[s], r0));
+    auto parts_of = [&](int pages, int len) { return (pages + len - 1) / len; };
+    auto fits = [&](int len) {
+        int64_t n = 0;
+        for (int pages : groups) n += parts_of(pages, len);
+        return n * nkv <= tree_workgroups(P.rw);
+    };
+    int lo = 1, hi = kPartPages / step;  // in rounds
+    while (lo < hi) {
+        const int mid = (lo + hi) / 2;
+        if (fits(mid * step))
+            hi = mid;
+        else
+            lo = mid + 1;
+    }
+    const int len = lo * step;
     for (int s = 0; cached && s < n_seqs; s++)
         for (int r0 = 0; r0 < in[s].n; r0 += P.rw * rps) {
             const RowSeq& q = in[s];
-            const int pages = group_pages(q, r0), parts = (int)((pages + len - 1) / len);
+            const int pages = group_pages(q, r0), parts = parts_of(pages, len);
             const int per = ((pages + parts - 1) / parts + step - 1) / step * step;
-            const int np = (pages + per - 1) / per, slots = std::min(P.rw, (q.n - r0 + rps - 1) / rps);
+            const int np = parts_of(pages, per), slots = std::min(P.rw, (q.n - r0 + rps - 1) / rps);
             for (int p = 0; p < np; p++) {
                 const int32_t rec[kItemWords] = {s, r0, p * per, std::min(pages, (p + 1) * per), P.n_wi + p, np, slots,
                                                  np == 1};
@@ -157,6 +172,15 @@ inline void plan_rows(RowPlan& P, const RowSeq* in, int n_seqs, int nh, int nkv,
         P.words += (n + 63) / 64 * 64;
         return r;
     };
+    // longest first: what is left at the end is short
+    std::vector<int> order(P.n_items);
+    for (int i = 0; i < P.n_items; i++) order[i] = i;
+    auto length = [&](int i) { return P.items[(size_t)i * kItemWords + 3] - P.items[(size_t)i * kItemWords + 2]; };
+    std::stable_sort(order.begin(), order.end(), [&](int a, int b) { return length(a) > length(b); });
+    std::vector<int32_t> sorted;
+    for (int i : order)
+        sorted.insert(sorted.end(), P.items.begin() + (size_t)i * kItemWords, P.items.begin() + (size_t)(i + 1) * kItemWords);
+    P.items.swap(sorted);
     // capacities in steps, so that the layout (and a captured step) lasts while contexts grow; the
     // added items and quads are unused
     P.n_items = (P.n_items + 15) / 16 * 16;

@@ -233,49 +233,62 @@ __device__ __forceinline__ void value_scales(const ValuePage<HD, FMT>& p, float 
     }
 }
 
-}  // namespace
+// An item's geometry, the same for all of its waves.
+struct Item {
+    int seq0, n, pos, btab, mask0, mpages;  // the sequence's record
+    int row0, page0, page1, wi, wi_step, slots, alone;
+    bool chain;
+    __device__ __forceinline__ bool read(const RowArgs& a, int item) {
+        const int4 i0 = *(const int4*)(a.items + (size_t)item * kItemWords),
+                   i1 = *(const int4*)(a.items + (size_t)item * kItemWords + 4);
+        if (i0.x < 0) return false;  // an unused item of the launch's capacity
+        const int32_t* s = a.seqs + (size_t)i0.x * kSeqWords;
+        const int4 s0 = *(const int4*)s, s1 = *(const int4*)(s + 4);
+        seq0 = s0.x, n = s0.y, pos = s0.z, btab = s0.w, mask0 = s1.x, mpages = s1.y;
+        chain = mask0 < 0;
+        row0 = i0.y, page0 = i0.z, page1 = i0.w, wi = i1.x, wi_step = i1.y, slots = i1.z, alone = i1.w;
+        return true;
+    }
+};
 
-// One workgroup per (kv head, item): rw row slots x pw position shares, a wave
-// each; the shares' sums meet in LDS.
+// A wave's slot: 16 QT queries of one kv head, and what they have gathered.
 template <int HD, int FMT, int QT>
-__global__ __launch_bounds__(512) void k_tree_attn(RowArgs a, KvLayer kv, TreeAttn t) {
-    constexpr int KD = HD / 16, NS = Keys<HD, FMT>::NS;
-    constexpr int QM = HD >= 64 ? 32 : 64;
-    constexpr bool F32 = FMT == KV_F32;
-    constexpr int ND = 4 * KD + 2;  // dwords a lane keeps of a tile
-    extern __shared__ float sh[];
-    const int h = blockIdx.x % kv.nkv, item = blockIdx.x / kv.nkv;
-    const int4 i0 = *(const int4*)(a.items + (size_t)item * kItemWords),
-               i1 = *(const int4*)(a.items + (size_t)item * kItemWords + 4);
-    if (i0.x < 0) return;  // an unused item of the launch's capacity
-    const int4 s0 = *(const int4*)(a.seqs + (size_t)i0.x * kSeqWords), s1 = *(const int4*)(a.seqs + (size_t)i0.x * kSeqWords + 4);
-    const int seq0 = s0.x, n = s0.y, pos = s0.z, btab = s0.w, mask0 = s1.x, mpages = s1.y;
-    const bool chain = mask0 < 0;
-    const int G = t.nh / kv.nkv, rps = QM / G;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
-    const int slot = wave % a.rw, share = wave / a.rw;
-    const int r0 = i0.y + slot * rps, nr = min(rps, n - r0), Q = nr * G;
-    const bool on = slot < i1.z && nr > 0;
-
+struct Slot {
+    static constexpr int KD = HD / 16, NS = Keys<HD, FMT>::NS, QM = HD >= 64 ? 32 : 64;
+    static constexpr int ND = 4 * KD + 2;  // dwords a lane keeps of a tile
+    static constexpr bool F32 = FMT == KV_F32;
     f16x8 qh[QT][NS], ql[QT][NS];
     float qf[QT], mq[QT], l[QT];  // score factor (log 2 units), reference, sum of probabilities
-    int qrow[QT];                          // the query's row in its sequence
+    int qrow[QT];                 // the query's row in its sequence
     f32x4 o[QT][KD];
+    int h, G, r0, nr, last, full;  // first row and rows; pages that they see; tokens that all of them see
+    bool on;
+
+    __device__ __forceinline__ void start(const RowArgs& a, const TreeAttn& t, const Item& it, int nkv, int head, int slot,
+                                          int lane) {
+        h = head;
+        G = t.nh / nkv;
+        r0 = it.row0 + slot * (QM / G);
+        nr = min(QM / G, it.n - r0);
+        on = slot < it.slots && nr > 0;
+        last = it.chain ? min(it.page1, (it.pos + r0 + nr + 15) / 16) : it.page1;
+        full = it.chain ? it.pos + r0 + 1 : it.pos;
 #pragma unroll
-    for (int i = 0; i < QT; i++) {
-        mq[i] = kLowest;
-        l[i] = 0.0f;
-        qf[i] = 1.0f;
-        qrow[i] = 0;
+        for (int i = 0; i < QT; i++) {
+            mq[i] = kLowest;
+            l[i] = 0.0f;
+            qf[i] = 1.0f;
+            qrow[i] = 0;
 #pragma unroll
-        for (int j = 0; j < KD; j++) o[i][j] = (f32x4){0, 0, 0, 0};
-    }
-    if (on) {
+            for (int j = 0; j < KD; j++) o[i][j] = (f32x4){0, 0, 0, 0};
+        }
+        if (!on) return;
+        const int r = lane & 15, g = lane >> 4, Q = nr * G;
 #pragma unroll
         for (int i = 0; i < QT; i++) {
             const int qi = min(16 * i + r, Q - 1);  // lanes past the last query hold it again
             qrow[i] = r0 + qi / G;
-            const int64_t row = seq0 + qrow[i];
+            const int64_t row = it.seq0 + qrow[i];
             const float* qp = t.q + row * t.ldq + (h * G + qi % G) * HD;
             float x[HD / 4];
 #pragma unroll
@@ -307,198 +320,332 @@ __global__ __launch_bounds__(512) void k_tree_attn(RowArgs a, KvLayer kv, TreeAt
                 split8(y, qh[i][s], ql[i][s]);
             }
         }
-        const int last = chain ? min(i0.w, (pos + r0 + nr + 15) / 16) : i0.w;  // pages that the slot's rows see
-        const int pairs = (last - i0.z + 1) / 2, mine = (pairs - share + a.pw - 1) / a.pw;
-        const int full = chain ? pos + r0 + 1 : pos;  // tokens that all of the slot's rows see
-        for (int c0 = 0; c0 < mine; c0 += 32) {
-            // the chunk's block ids, two pages a pair; past the last page the last again
-            const int pg = i0.z + 2 * (share + a.pw * (c0 + lane / 2)) + (lane & 1);
-            const int ids = a.btab[btab + min(pg, last - 1)];
-            const int np = min(32, mine - c0);
-            // keys and values are asked for as soon as the registers of the pair before are free: the keys behind
-            // the scores, the values behind the weighted sum
-            KeyPage<HD, FMT> kp[2];
-            ValuePage<HD, FMT> vp[2];
-            auto block = [&](int c, int x) { return (size_t)(uint32_t)__builtin_amdgcn_readlane(ids, 2 * c + x); };
-#pragma unroll
-            for (int x = 0; x < 2; x++) kp[x].load(kv, block(0, x), h, lane);
-#pragma unroll
-            for (int x = 0; x < 2; x++) vp[x].load(kv, block(0, x), h, lane);
-            for (int c = 0; c < np; c++) {
-                const int p0 = i0.z + 2 * (share + a.pw * (c0 + c));  // the pair's first page
-                const int next = min(c + 1, np - 1);
-                float raw[2][QT][4];
-#pragma unroll
-                for (int x = 0; x < 2; x++) {
-                    const Keys<HD, FMT> k(kp[x], lane);
-#pragma unroll
-                    for (int i = 0; i < QT; i++) {
-                        f32x4 acc = (f32x4){0, 0, 0, 0};
-#pragma unroll
-                        for (int s = 0; s < NS; s++) {
-                            acc = mfma(k.hi[s], ql[i][s], acc);
-                            if constexpr (F32) acc = mfma(k.lo[s], qh[i][s], acc);
-                            acc = mfma(k.hi[s], qh[i][s], acc);
-                        }
-#pragma unroll
-                        for (int e = 0; e < 4; e++) raw[x][i][e] = acc[e] * k.s[e];
-                    }
-                }
-#pragma unroll
-                for (int x = 0; x < 2; x++) kp[x].load(kv, block(next, x), h, lane);
-                if (16 * (p0 + 2) > full || p0 + 1 >= last) {
-#pragma unroll
-                    for (int x = 0; x < 2; x++)
-#pragma unroll
-                        for (int i = 0; i < QT; i++) {
-                            const int page = p0 + x, at = 16 * page + 4 * g;
-                            uint32_t sees = page < last ? 15u : 0u;
-                            if (chain)
-                                sees &= at > pos + qrow[i] ? 0u : 15u >> max(0, 3 - (pos + qrow[i] - at));
-                            else if (page >= pos / 16 && page < last)
-                                sees &= (uint32_t)a.masks[mask0 + (size_t)qrow[i] * mpages + (page - pos / 16)] >> (4 * g);
-#pragma unroll
-                            for (int e = 0; e < 4; e++) raw[x][i][e] = sees >> e & 1 ? raw[x][i][e] : -INFINITY;
-                        }
-                }
-                float vsc[2][4], vf[2][4];
-#pragma unroll
-                for (int x = 0; x < 2; x++) value_scales<HD, FMT>(vp[x], vsc[x], vf[x]);
-                uint32_t ph[QT][4], pl[QT][4];
-#pragma unroll
-                for (int i = 0; i < QT; i++) {
-                    float p[8], w[8];
-                    auto weigh = [&] {
-#pragma unroll
-                        for (int x = 0; x < 2; x++)
-#pragma unroll
-                            for (int e = 0; e < 4; e++) {
-                                const float y = __builtin_amdgcn_exp2f(fmaf(raw[x][i][e], qf[i], -mq[i]));
-                                p[4 * x + e] = y;
-                                w[4 * x + e] = y * vsc[x][e];
-                            }
-                    };
-                    weigh();
-                    float wm = 0.0f, pm = 0.0f;
-#pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        wm = fmaxf(wm, w[e]);
-                        pm = fmaxf(pm, p[e]);
-                    }
-                    if (__any(wm > kMost || pm > kMostP)) {
-                        float top = -INFINITY;
-#pragma unroll
-                        for (int x = 0; x < 2; x++)
-#pragma unroll
-                            for (int e = 0; e < 4; e++) {
-                                const float sc = raw[x][i][e] * qf[i];
-                                top = fmaxf(top, fmaxf(sc + __builtin_amdgcn_logf(vsc[x][e]) - kTop, sc - kTopP));
-                            }
-                        const float mn = fmaxf(mq[i], reduce_rows<true, true>(top)), f = __builtin_amdgcn_exp2f(mq[i] - mn);
-                        l[i] *= f;
-#pragma unroll
-                        for (int j = 0; j < KD; j++) o[i][j] *= f;
-                        mq[i] = mn;
-                        weigh();
-                    }
-                    // a value that is not finite has a NaN scale, which must not reach the rows that don't see it
-#pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        l[i] += p[e];
-                        w[e] = p[e] == 0.0f ? 0.0f : w[e];
-                    }
-#pragma unroll
-                    for (int e = 0; e < 4; e++) split2(w[2 * e], w[2 * e + 1], ph[i][e], pl[i][e]);
-                }
-#pragma unroll
-                for (int j = 0; j < KD; j++) {
-                    f16x8 vh, vl;
-                    if constexpr (F32) {
-                        float y[8];
-#pragma unroll
-                        for (int x = 0; x < 2; x++)
-#pragma unroll
-                            for (int e = 0; e < 4; e++) y[4 * x + e] = vf[x][e] == 0.0f ? 0.0f : vp[x].d[e][j] * vf[x][e];
-                        split8(y, vh, vl);
-                    } else {
-                        vh = codes8<FMT>(vp[0].d[j], vp[1].d[j]);
-                    }
-#pragma unroll
-                    for (int i = 0; i < QT; i++) {
-                        const f16x8 hi = __builtin_bit_cast(f16x8, (u32x4){ph[i][0], ph[i][1], ph[i][2], ph[i][3]});
-                        const f16x8 lo = __builtin_bit_cast(f16x8, (u32x4){pl[i][0], pl[i][1], pl[i][2], pl[i][3]});
-                        o[i][j] = mfma(vh, lo, o[i][j]);
-                        if constexpr (F32) o[i][j] = mfma(vl, hi, o[i][j]);
-                        o[i][j] = mfma(vh, hi, o[i][j]);
-                    }
-                }
-#pragma unroll
-                for (int x = 0; x < 2; x++) vp[x].load(kv, block(next, x), h, lane);
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < QT; i++) l[i] = reduce_rows<false, true>(l[i]);
     }
-    // the position shares, halved until one holds the sums; a tile at a time, for the LDS that takes
-    for (int half = a.pw / 2; half > 0; half >>= 1) {
-        float* x = sh + ((size_t)(share % half * a.rw + slot) * ND) * 64 + lane;
+
+    // Scores of a page: raw[tile][token], to be multiplied by qf.
+    __device__ __forceinline__ void scores(const KeyPage<HD, FMT>& p, float (&raw)[QT][4], int lane) const {
+        const Keys<HD, FMT> k(p, lane);
 #pragma unroll
         for (int i = 0; i < QT; i++) {
-            if (on && share >= half && share < 2 * half) {
-                x[0] = mq[i];
-                x[64] = l[i];
+            f32x4 acc = (f32x4){0, 0, 0, 0};
 #pragma unroll
-                for (int j = 0; j < KD; j++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) x[(2 + 4 * j + e) * 64] = o[i][j][e];
+            for (int s = 0; s < NS; s++) {
+                acc = mfma(k.hi[s], ql[i][s], acc);
+                if constexpr (F32) acc = mfma(k.lo[s], qh[i][s], acc);
+                acc = mfma(k.hi[s], qh[i][s], acc);
             }
-            __syncthreads();
-            if (on && share < half) {
-                const float m2 = x[0], mn = fmaxf(mq[i], m2);
-                const float f1 = __builtin_amdgcn_exp2f(mq[i] - mn), f2 = __builtin_amdgcn_exp2f(m2 - mn);
-                l[i] = l[i] * f1 + x[64] * f2;
 #pragma unroll
-                for (int j = 0; j < KD; j++)
+            for (int e = 0; e < 4; e++) raw[i][e] = acc[e] * k.s[e];
+        }
+    }
+
+    // Whether some query does not see all of a pair of pages.
+    __device__ __forceinline__ bool masked(int p0) const { return 16 * (p0 + 2) > full || p0 + 1 >= last; }
+    __device__ __forceinline__ void mask(const RowArgs& a, const Item& it, int page, float (&raw)[QT][4], int lane) const {
+        const int g = lane >> 4, at = 16 * page + 4 * g;
 #pragma unroll
-                    for (int e = 0; e < 4; e++) o[i][j][e] = o[i][j][e] * f1 + x[(2 + 4 * j + e) * 64] * f2;
+        for (int i = 0; i < QT; i++) {
+            uint32_t sees = page < last ? 15u : 0u;
+            const int end = it.pos + qrow[i];  // of a chain's row: the last token that it sees
+            if (it.chain)
+                sees &= at > end ? 0u : 15u >> max(0, 3 - (end - at));
+            else if (page >= it.pos / 16 && page < last)
+                sees &= (uint32_t)a.masks[it.mask0 + (size_t)qrow[i] * it.mpages + (page - it.pos / 16)] >> (4 * g);
+#pragma unroll
+            for (int e = 0; e < 4; e++) raw[i][e] = sees >> e & 1 ? raw[i][e] : -INFINITY;
+        }
+    }
+
+    // Weights of a pair of pages' tokens (raw[page]), and their values.
+    __device__ __forceinline__ void gather(const float (&raw)[2][QT][4], const ValuePage<HD, FMT> (&vp)[2]) {
+        float vsc[2][4], vf[2][4];
+#pragma unroll
+        for (int x = 0; x < 2; x++) value_scales<HD, FMT>(vp[x], vsc[x], vf[x]);
+        uint32_t ph[QT][4], pl[QT][4];
+#pragma unroll
+        for (int i = 0; i < QT; i++) {
+            float p[8], w[8];
+            auto weigh = [&] {
+#pragma unroll
+                for (int x = 0; x < 2; x++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const float y = __builtin_amdgcn_exp2f(fmaf(raw[x][i][e], qf[i], -mq[i]));
+                        p[4 * x + e] = y;
+                        w[4 * x + e] = y * vsc[x][e];
+                    }
+            };
+            weigh();
+            float wm = 0.0f, pm = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                wm = fmaxf(wm, w[e]);
+                pm = fmaxf(pm, p[e]);
+            }
+            if (__any(wm > kMost || pm > kMostP)) {
+                float top = -INFINITY;
+#pragma unroll
+                for (int x = 0; x < 2; x++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const float sc = raw[x][i][e] * qf[i];
+                        top = fmaxf(top, fmaxf(sc + __builtin_amdgcn_logf(vsc[x][e]) - kTop, sc - kTopP));
+                    }
+                const float mn = fmaxf(mq[i], reduce_rows<true, true>(top)), f = __builtin_amdgcn_exp2f(mq[i] - mn);
+                l[i] *= f;
+#pragma unroll
+                for (int j = 0; j < KD; j++) o[i][j] *= f;
                 mq[i] = mn;
+                weigh();
             }
-            __syncthreads();
+            // a value that is not finite has a NaN scale, which must not reach the rows that don't see it
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                l[i] += p[e];
+                w[e] = p[e] == 0.0f ? 0.0f : w[e];
+            }
+#pragma unroll
+            for (int e = 0; e < 4; e++) split2(w[2 * e], w[2 * e + 1], ph[i][e], pl[i][e]);
+        }
+#pragma unroll
+        for (int j = 0; j < KD; j++) {
+            f16x8 vh, vl;
+            if constexpr (F32) {
+                float y[8];
+#pragma unroll
+                for (int x = 0; x < 2; x++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) y[4 * x + e] = vf[x][e] == 0.0f ? 0.0f : vp[x].d[e][j] * vf[x][e];
+                split8(y, vh, vl);
+            } else {
+                vh = codes8<FMT>(vp[0].d[j], vp[1].d[j]);
+            }
+#pragma unroll
+            for (int i = 0; i < QT; i++) {
+                const f16x8 hi = __builtin_bit_cast(f16x8, (u32x4){ph[i][0], ph[i][1], ph[i][2], ph[i][3]});
+                const f16x8 lo = __builtin_bit_cast(f16x8, (u32x4){pl[i][0], pl[i][1], pl[i][2], pl[i][3]});
+                o[i][j] = mfma(vh, lo, o[i][j]);
+                if constexpr (F32) o[i][j] = mfma(vl, hi, o[i][j]);
+                o[i][j] = mfma(vh, hi, o[i][j]);
+            }
         }
     }
-    if (!on || share != 0) return;
+
+    // The sums of the pw position shares into share 0's, halving; a tile at a time, for the LDS that takes. Every
+    // wave of the workgroup calls it; sh: pw / 2 * rw * ND * 64 floats.
+    __device__ __forceinline__ void join(float* sh, int slot, int share, int rw, int pw, int lane) {
 #pragma unroll
-    for (int i = 0; i < QT; i++) {
-        const int qi = 16 * i + r;
-        if (qi >= Q) continue;
-        float* dst;
-        float f = 1.0f;
-        if (t.out && i1.w) {
-            // no other item has these rows: what they attend to, zeros where that is nothing
-            const bool none = l[i] == 0.0f || a.mrec[(size_t)(seq0 + qrow[i]) * 4 + 3];
-            f = none ? 0.0f : 1.0f / l[i];
-            if (none) {
+        for (int i = 0; i < QT; i++) l[i] = reduce_rows<false, true>(l[i]);
+        for (int half = pw / 2; half > 0; half >>= 1) {
+            float* x = sh + ((size_t)(share % half * rw + slot) * ND) * 64 + lane;
 #pragma unroll
-                for (int j = 0; j < KD; j++) o[i][j] = (f32x4){0, 0, 0, 0};
+            for (int i = 0; i < QT; i++) {
+                if (on && share >= half && share < 2 * half) {
+                    x[0] = mq[i];
+                    x[64] = l[i];
+#pragma unroll
+                    for (int j = 0; j < KD; j++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) x[(2 + 4 * j + e) * 64] = o[i][j][e];
+                }
+                __syncthreads();
+                if (on && share < half) {
+                    const float m2 = x[0], mn = fmaxf(mq[i], m2);
+                    const float f1 = __builtin_amdgcn_exp2f(mq[i] - mn), f2 = __builtin_amdgcn_exp2f(m2 - mn);
+                    l[i] = l[i] * f1 + x[64] * f2;
+#pragma unroll
+                    for (int j = 0; j < KD; j++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) o[i][j][e] = o[i][j][e] * f1 + x[(2 + 4 * j + e) * 64] * f2;
+                    mq[i] = mn;
+                }
+                __syncthreads();
             }
-            dst = t.out + (size_t)(seq0 + qrow[i]) * t.ldo + (size_t)(h * G + qi % G) * HD;
-        } else {
-            float* part = t.part + (((size_t)(i1.x + slot * i1.y) * kv.nkv + h) * QM + qi) * (HD + 4);
-            if (g == 0) {
-                part[0] = l[i] == 0.0f ? -INFINITY : t.out ? mq[i] : mq[i] * kLn2;
-                part[1] = l[i];
-            }
-            dst = part + 4;
-        }
-        dst += g * (HD / 4);
-#pragma unroll
-        for (int w = 0; w < KD; w++) {  // channel 4 w + e of the lane's: tile (4 w + e) % KD, register (4 w + e) / KD
-            f32x4 y;
-#pragma unroll
-            for (int e = 0; e < 4; e++) y[e] = o[i][(4 * w + e) % KD][(4 * w + e) / KD] * f;
-            *(f32x4*)(dst + 4 * w) = y;
         }
     }
+
+    // Share 0: the outputs of rows that no other item has, partials of the others'.
+    __device__ __forceinline__ void finish(const RowArgs& a, const TreeAttn& t, const Item& it, int nkv, int slot,
+                                           int lane) {
+        const int r = lane & 15, g = lane >> 4;
+#pragma unroll
+        for (int i = 0; i < QT; i++) {
+            const int qi = 16 * i + r;
+            if (qi >= nr * G) continue;
+            float* dst;
+            float f = 1.0f;
+            if (t.out && it.alone) {
+                // zeros where a row attends to nothing
+                const bool none = l[i] == 0.0f || a.mrec[(size_t)(it.seq0 + qrow[i]) * 4 + 3];
+                f = none ? 0.0f : 1.0f / l[i];
+                if (none) {
+#pragma unroll
+                    for (int j = 0; j < KD; j++) o[i][j] = (f32x4){0, 0, 0, 0};
+                }
+                dst = t.out + (size_t)(it.seq0 + qrow[i]) * t.ldo + (size_t)(h * G + qi % G) * HD;
+            } else {
+                float* part = t.part + (((size_t)(it.wi + slot * it.wi_step) * nkv + h) * QM + qi) * (HD + 4);
+                if (g == 0) {
+                    part[0] = l[i] == 0.0f ? -INFINITY : t.out ? mq[i] : mq[i] * kLn2;
+                    part[1] = l[i];
+                }
+                dst = part + 4;
+            }
+            dst += g * (HD / 4);
+#pragma unroll
+            for (int w = 0; w < KD; w++) {  // channel 4 w + e of the lane's: tile (4 w + e) % KD, register (4 w + e) / KD
+                f32x4 y;
+#pragma unroll
+                for (int e = 0; e < 4; e++) y[e] = o[i][(4 * w + e) % KD][(4 * w + e) / KD] * f;
+                *(f32x4*)(dst + 4 * w) = y;
+            }
+        }
+    }
+};
+
+}  // namespace
+
+// One workgroup per (kv head, item): rw row slots x pw position shares, a wave
+// each, which takes its pages from memory straight to registers; the shares'
+// sums meet in LDS.
+template <int HD, int FMT, int QT>
+__global__ __launch_bounds__(512) void k_tree_attn(RowArgs a, KvLayer kv, TreeAttn t) {
+    extern __shared__ float sh[];
+    Item it;
+    if (!it.read(a, blockIdx.x / kv.nkv)) return;
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // what depends on it stays scalar
+    const int slot = wave % a.rw, share = wave / a.rw;
+    Slot<HD, FMT, QT> s;
+    s.start(a, t, it, kv.nkv, blockIdx.x % kv.nkv, slot, lane);
+    const int pairs = (s.last - it.page0 + 1) / 2, mine = s.on ? (pairs - share + a.pw - 1) / a.pw : 0;
+    for (int c0 = 0; c0 < mine; c0 += 32) {
+        // the chunk's block ids, two pages a pair; past the last page the last again
+        const int pg = it.page0 + 2 * (share + a.pw * (c0 + lane / 2)) + (lane & 1);
+        const int ids = a.btab[it.btab + min(pg, s.last - 1)];
+        const int np = min(32, mine - c0);
+        auto block = [&](int c, int x) { return (size_t)(uint32_t)__builtin_amdgcn_readlane(ids, 2 * c + x); };
+        // keys and values are asked for as soon as the registers of the pair before are free: the keys behind
+        // the scores, the values behind the weighted sum
+        KeyPage<HD, FMT> kp[2];
+        ValuePage<HD, FMT> vp[2];
+#pragma unroll
+        for (int x = 0; x < 2; x++) kp[x].load(kv, block(0, x), s.h, lane);
+#pragma unroll
+        for (int x = 0; x < 2; x++) vp[x].load(kv, block(0, x), s.h, lane);
+        for (int c = 0; c < np; c++) {
+            const int p0 = it.page0 + 2 * (share + a.pw * (c0 + c));  // the pair's first page
+            const int next = min(c + 1, np - 1);
+            float raw[2][QT][4];
+#pragma unroll
+            for (int x = 0; x < 2; x++) s.scores(kp[x], raw[x], lane);
+#pragma unroll
+            for (int x = 0; x < 2; x++) kp[x].load(kv, block(next, x), s.h, lane);
+            if (s.masked(p0))
+#pragma unroll
+                for (int x = 0; x < 2; x++) s.mask(a, it, p0 + x, raw[x], lane);
+            s.gather(raw, vp);
+#pragma unroll
+            for (int x = 0; x < 2; x++) vp[x].load(kv, block(next, x), s.h, lane);
+        }
+    }
+    s.join(sh, slot, share, a.rw, a.pw, lane);
+    if (s.on && share == 0) s.finish(a, t, it, kv.nkv, slot, lane);
+}
+
+// The same for sequences of several slots over 8-bit caches: the slots' waves
+// take each page once, through LDS. A ring of stages (a pair of pages for every
+// position share) is filled by copies from memory straight to LDS, NST - 1 stages ahead, so
+// that enough bytes are on their way to cover the latency of memory: with every
+// wave loading for itself a CU asks for the same 17 KB four times. 16-byte
+// chunks lie in LDS by (chunk, row) so that 16 lanes read 256 consecutive bytes.
+template <int HD, int FMT, int RW>
+__global__ __launch_bounds__(512) void k_tree_attn_lds(RowArgs a, KvLayer kv, TreeAttn t) {
+    constexpr int QT = 2, PW = RW == 2 ? 4 : 2, W = RW * PW, CPR = HD / 64;  // CPR: 16-byte chunks a lane takes of a page
+    constexpr int REC = 32 * HD + 128, STAGE = 2 * PW * REC, NST = RW == 2 ? 4 : 7;
+    constexpr int COPIES = (2 * PW * 2 * CPR + W - 1) / W;  // 1 KB copies a wave makes of a stage's codes
+    constexpr int JOIN = PW / 2 * RW * Slot<HD, FMT, QT>::ND * 64 * 4;
+    static_assert(HD == 64 || HD == 128, "whole chunks");
+    static_assert(W <= 8 && NST * STAGE + 4 * kPartPages <= 160 * 1024 && JOIN <= NST * STAGE, "a CU's LDS");
+    __shared__ __align__(1024) uint8_t ring[NST * STAGE];
+    __shared__ int32_t ids[kPartPages];
+    Item it;
+    if (!it.read(a, blockIdx.x / kv.nkv)) return;
+    const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int slot = wave % RW, share = wave / RW;
+    const int pages = it.page1 - it.page0, stages = (pages + 2 * PW - 1) / (2 * PW);
+    for (int i = threadIdx.x; i < pages; i += 64 * W) ids[i] = a.btab[it.btab + it.page0 + i];
+    Slot<HD, FMT, QT> s;
+    s.start(a, t, it, kv.nkv, blockIdx.x % kv.nkv, slot, lane);
+    __syncthreads();
+    // the wave's copies of a stage: codes copy i of page `page`, from byte `off` of its record to byte `to` of the
+    // stage; more copies than there are repeat the last
+    uint32_t off[COPIES];
+    int page[COPIES], to[COPIES];
+#pragma unroll
+    for (int i = 0; i < COPIES; i++) {
+        const int q = min(wave + W * i, 2 * PW * 2 * CPR - 1), part = q % (2 * CPR), c = (part % CPR * 64 + lane) / 16;
+        page[i] = q / (2 * CPR);
+        to[i] = page[i] * REC + part * 1024;
+        off[i] = part < CPR ? r * HD + c * 16 : 16 * HD + c / CPR * (4 * HD) + r * (HD / 4) + c % CPR * 16;
+    }
+    const int spage = wave % (2 * PW);  // and the scales of a page
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)ring;
+    auto record = [&](int stage, int pg) {  // past the last page the last again
+        const uint32_t id = __builtin_amdgcn_readfirstlane(ids[min(stage * 2 * PW + pg, pages - 1)]);
+        return kv.data + ((size_t)id * kv.nkv + s.h) * REC;
+    };
+    auto copy = [&](int stage) {
+        const uint32_t at = lds0 + stage % NST * STAGE;
+#pragma unroll
+        for (int i = 0; i < COPIES; i++) copy_to_lds(at + to[i], record(stage, page[i]), off[i]);
+        if (lane < 8) copy_to_lds(at + spage * REC + 32 * HD, record(stage, spage) + 32 * HD, 16 * lane);
+    };
+    for (int i = 0; i < NST - 1; i++) copy(i);
+    for (int st = 0; st < stages; st++) {
+        // this wave's copies of the stage have landed, then everyone's; and everyone has left the stage that the next
+        // copies overwrite
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NST - 2) * (COPIES + 1)) : "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        copy(st + NST - 1);
+        const int p0 = it.page0 + 2 * (share + PW * st);
+        if (!s.on || p0 >= s.last) continue;
+        const uint8_t* base = ring + st % NST * STAGE + 2 * share * REC;
+        float raw[2][QT][4];
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+            KeyPage<HD, FMT> k;
+#pragma unroll
+            for (int j = 0; j < CPR; j++) {
+                const u32x4 y = *(const u32x4*)(base + x * REC + ((g * CPR + j) * 16 + r) * 16);
+#pragma unroll
+                for (int e = 0; e < 4; e++) k.d[4 * j + e] = y[e];
+            }
+            k.s = *(const float4*)(base + x * REC + 32 * HD + 16 * g);
+            s.scores(k, raw[x], lane);
+        }
+        if (s.masked(p0))
+#pragma unroll
+            for (int x = 0; x < 2; x++) s.mask(a, it, p0 + x, raw[x], lane);
+        ValuePage<HD, FMT> v[2];
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+#pragma unroll
+            for (int j = 0; j < CPR; j++) {
+                const u32x4 y = *(const u32x4*)(base + x * REC + 16 * HD + ((g * CPR + j) * 16 + r) * 16);
+#pragma unroll
+                for (int e = 0; e < 4; e++) v[x].d[4 * j + e] = y[e];
+            }
+            v[x].s = *(const float4*)(base + x * REC + 32 * HD + 64 + 16 * g);
+        }
+        s.gather(raw, v);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no copy is left on its way when the ring is reused, or given up
+    __syncthreads();
+    s.join((float*)ring, slot, share, RW, PW, lane);
+    if (s.on && share == 0) s.finish(a, t, it, kv.nkv, slot, lane);
 }
 
 // The parts of each row's heads: one workgroup per (row, kv head x QH heads),
@@ -558,12 +705,24 @@ __global__ __launch_bounds__(256) void k_tree_merge(RowArgs a, TreeAttn t, int n
 template <int HD, int FMT>
 static void tree_qt(hipStream_t st, const RowArgs& a, const KvLayer& kv, const TreeAttn& t) {
     const dim3 grid((unsigned)kv.nkv * a.n_items), block(64 * a.rw * a.pw);
-    const size_t per = (size_t)64 * 4 * (4 * (HD / 16) + 2) * (a.pw / 2) * a.rw;
     constexpr int QT = HD >= 64 ? 2 : 4;
+    if constexpr (HD >= 64 && FMT != KV_F32) {
+        // several slots, which then hold more than 16 queries each
+        if (a.rw > 1) {
+            if (a.rw == 2)
+                hipLaunchKernelGGL((k_tree_attn_lds<HD, FMT, 2>), grid, block, 0, st, a, kv, t);
+            else if (a.rw == 3)
+                hipLaunchKernelGGL((k_tree_attn_lds<HD, FMT, 3>), grid, block, 0, st, a, kv, t);
+            else
+                hipLaunchKernelGGL((k_tree_attn_lds<HD, FMT, 4>), grid, block, 0, st, a, kv, t);
+            return;
+        }
+    }
+    const size_t join = (size_t)64 * 4 * Slot<HD, FMT, QT>::ND * (a.pw / 2) * a.rw;
     if (a.qt == 1)
-        hipLaunchKernelGGL((k_tree_attn<HD, FMT, 1>), grid, block, per, st, a, kv, t);
+        hipLaunchKernelGGL((k_tree_attn<HD, FMT, 1>), grid, block, join, st, a, kv, t);
     else
-        hipLaunchKernelGGL((k_tree_attn<HD, FMT, QT>), grid, block, per, st, a, kv, t);
+        hipLaunchKernelGGL((k_tree_attn<HD, FMT, QT>), grid, block, join, st, a, kv, t);
 }
 
 template <int HD>
