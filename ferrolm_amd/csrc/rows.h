@@ -128,7 +128,7 @@ inline void plan_rows(RowPlan& P, const RowSeq* in, int n_seqs, int nh, int nkv,
         return (last + 15) / 16;
     };
     // the shortest parts, in whole rounds of a workgroup's waves, that make no more workgroups than that
-    const int step = 2 * P.pw;
+    const int step = P.rw > 1 ? 4 * P.pw : 2 * P.pw;
     std::vector<int> groups;  // pages of every row group
     for (int s = 0; cached && s < n_seqs; s++)
         for (int r0 = 0; r0 < in[s].n; r0 += P.rw * rps) groups.push_back(group_pages(in[s], r0));

@@ -216,7 +216,7 @@ struct Keys {
 
 // Scales of the lane's four values of a page, and for f32 the factors to split them by (0: not finite).
 template <int HD, int FMT>
-__device__ __forceinline__ void value_scales(const ValuePage<HD, FMT>& p, float (&s)[4], float (&f)[4]) {
+__device__ __forceinline__ void value_scales(const ValuePage<HD, FMT>& p, float* s, float* f) {
     if constexpr (FMT == KV_F32) {
 #pragma unroll
         for (int t = 0; t < 4; t++) {
@@ -322,111 +322,120 @@ struct Slot {
         }
     }
 
-    // Scores of a page: raw[tile][token], to be multiplied by qf.
-    __device__ __forceinline__ void scores(const KeyPage<HD, FMT>& p, float (&raw)[QT][4], int lane) const {
-        const Keys<HD, FMT> k(p, lane);
+    // Scores of a pair of pages: raw[tile][page x 4 tokens], to be multiplied by qf. Products into one sum stand
+    // apart, by the pages' and tiles' others.
+    __device__ __forceinline__ void scores(const KeyPage<HD, FMT> (&kp)[2], float (&raw)[QT][8], int lane) const {
+        const Keys<HD, FMT> k[2] = {Keys<HD, FMT>(kp[0], lane), Keys<HD, FMT>(kp[1], lane)};
+        f32x4 acc[2][QT];
 #pragma unroll
-        for (int i = 0; i < QT; i++) {
-            f32x4 acc = (f32x4){0, 0, 0, 0};
+        for (int x = 0; x < 2; x++)
 #pragma unroll
-            for (int s = 0; s < NS; s++) {
-                acc = mfma(k.hi[s], ql[i][s], acc);
-                if constexpr (F32) acc = mfma(k.lo[s], qh[i][s], acc);
-                acc = mfma(k.hi[s], qh[i][s], acc);
+            for (int i = 0; i < QT; i++) acc[x][i] = (f32x4){0, 0, 0, 0};
+#pragma unroll
+        for (int s = 0; s < NS; s++) {
+#pragma unroll
+            for (int x = 0; x < 2; x++)
+#pragma unroll
+                for (int i = 0; i < QT; i++) acc[x][i] = mfma(k[x].hi[s], ql[i][s], acc[x][i]);
+            if constexpr (F32) {
+#pragma unroll
+                for (int x = 0; x < 2; x++)
+#pragma unroll
+                    for (int i = 0; i < QT; i++) acc[x][i] = mfma(k[x].lo[s], qh[i][s], acc[x][i]);
             }
 #pragma unroll
-            for (int e = 0; e < 4; e++) raw[i][e] = acc[e] * k.s[e];
+            for (int x = 0; x < 2; x++)
+#pragma unroll
+                for (int i = 0; i < QT; i++) acc[x][i] = mfma(k[x].hi[s], qh[i][s], acc[x][i]);
         }
+#pragma unroll
+        for (int x = 0; x < 2; x++)
+#pragma unroll
+            for (int i = 0; i < QT; i++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) raw[i][4 * x + e] = acc[x][i][e] * k[x].s[e];
     }
 
     // Whether some query does not see all of a pair of pages.
     __device__ __forceinline__ bool masked(int p0) const { return 16 * (p0 + 2) > full || p0 + 1 >= last; }
-    __device__ __forceinline__ void mask(const RowArgs& a, const Item& it, int page, float (&raw)[QT][4], int lane) const {
-        const int g = lane >> 4, at = 16 * page + 4 * g;
+
+    // Scores of tokens that tile i's query does not see: -infinity.
+    __device__ __forceinline__ void mask(const RowArgs& a, const Item& it, int p0, int i, float (&raw)[8], int lane) const {
 #pragma unroll
-        for (int i = 0; i < QT; i++) {
+        for (int x = 0; x < 2; x++) {
+            const int page = p0 + x, at = 16 * page + 4 * (lane >> 4), end = it.pos + qrow[i];  // end: a chain row's last
             uint32_t sees = page < last ? 15u : 0u;
-            const int end = it.pos + qrow[i];  // of a chain's row: the last token that it sees
             if (it.chain)
                 sees &= at > end ? 0u : 15u >> max(0, 3 - (end - at));
             else if (page >= it.pos / 16 && page < last)
-                sees &= (uint32_t)a.masks[it.mask0 + (size_t)qrow[i] * it.mpages + (page - it.pos / 16)] >> (4 * g);
+                sees &= (uint32_t)a.masks[it.mask0 + (size_t)qrow[i] * it.mpages + (page - it.pos / 16)] >> (lane >> 4 << 2);
 #pragma unroll
-            for (int e = 0; e < 4; e++) raw[i][e] = sees >> e & 1 ? raw[i][e] : -INFINITY;
+            for (int e = 0; e < 4; e++) raw[4 * x + e] = sees >> e & 1 ? raw[4 * x + e] : -INFINITY;
         }
     }
 
-    // Weights of a pair of pages' tokens (raw[page]), and their values.
-    __device__ __forceinline__ void gather(const float (&raw)[2][QT][4], const ValuePage<HD, FMT> (&vp)[2]) {
-        float vsc[2][4], vf[2][4];
-#pragma unroll
-        for (int x = 0; x < 2; x++) value_scales<HD, FMT>(vp[x], vsc[x], vf[x]);
-        uint32_t ph[QT][4], pl[QT][4];
+    // The pair p0's weights, in two f16 each, from its scores and value scales; the reference and sums follow.
+    __device__ __forceinline__ void weights(const RowArgs& a, const Item& it, int p0, float (&raw)[QT][8],
+                                            const float (&vsc)[8], f16x8 (&hi)[QT], f16x8 (&lo)[QT], int lane) {
+        const bool part = masked(p0);
 #pragma unroll
         for (int i = 0; i < QT; i++) {
             float p[8], w[8];
-            auto weigh = [&] {
+            auto weigh = [&] {  // true in a lane whose weights or probabilities are out of bounds
+                float wm = 0.0f, pm = 0.0f;
 #pragma unroll
-                for (int x = 0; x < 2; x++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const float y = __builtin_amdgcn_exp2f(fmaf(raw[x][i][e], qf[i], -mq[i]));
-                        p[4 * x + e] = y;
-                        w[4 * x + e] = y * vsc[x][e];
-                    }
+                for (int e = 0; e < 8; e++) {
+                    p[e] = __builtin_amdgcn_exp2f(fmaf(raw[i][e], qf[i], -mq[i]));
+                    w[e] = p[e] * vsc[e];
+                    wm = fmaxf(wm, w[e]);
+                    pm = fmaxf(pm, p[e]);
+                }
+                return wm > kMost || pm > kMostP;
             };
-            weigh();
-            float wm = 0.0f, pm = 0.0f;
+            if (__any(part | weigh())) {
+                if (part) mask(a, it, p0, i, raw[i], lane);
+                if (__any(weigh())) {
+                    float top = -INFINITY;
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                wm = fmaxf(wm, w[e]);
-                pm = fmaxf(pm, p[e]);
-            }
-            if (__any(wm > kMost || pm > kMostP)) {
-                float top = -INFINITY;
-#pragma unroll
-                for (int x = 0; x < 2; x++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const float sc = raw[x][i][e] * qf[i];
-                        top = fmaxf(top, fmaxf(sc + __builtin_amdgcn_logf(vsc[x][e]) - kTop, sc - kTopP));
+                    for (int e = 0; e < 8; e++) {
+                        const float sc = raw[i][e] * qf[i];
+                        top = fmaxf(top, fmaxf(sc + __builtin_amdgcn_logf(vsc[e]) - kTop, sc - kTopP));
                     }
-                const float mn = fmaxf(mq[i], reduce_rows<true, true>(top)), f = __builtin_amdgcn_exp2f(mq[i] - mn);
-                l[i] *= f;
+                    const float mn = fmaxf(mq[i], reduce_rows<true, true>(top)), f = __builtin_amdgcn_exp2f(mq[i] - mn);
+                    l[i] *= f;
 #pragma unroll
-                for (int j = 0; j < KD; j++) o[i][j] *= f;
-                mq[i] = mn;
-                weigh();
+                    for (int j = 0; j < KD; j++) o[i][j] *= f;
+                    mq[i] = mn;
+                    (void)weigh();
+                }
+                // a value that is not finite has a NaN scale, which must not reach the rows that don't see it
+#pragma unroll
+                for (int e = 0; e < 8; e++) w[e] = p[e] == 0.0f ? 0.0f : w[e];
             }
-            // a value that is not finite has a NaN scale, which must not reach the rows that don't see it
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                l[i] += p[e];
-                w[e] = p[e] == 0.0f ? 0.0f : w[e];
-            }
-#pragma unroll
-            for (int e = 0; e < 4; e++) split2(w[2 * e], w[2 * e + 1], ph[i][e], pl[i][e]);
+            split8(w, hi[i], lo[i]);
+            l[i] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
         }
+    }
+
+    // Adds a pair's weighted values; vf: value_scales' factors.
+    __device__ __forceinline__ void gather(const f16x8 (&hi)[QT], const f16x8 (&lo)[QT], const ValuePage<HD, FMT> (&vp)[2],
+                                           const float (&vf)[8]) {
 #pragma unroll
         for (int j = 0; j < KD; j++) {
             f16x8 vh, vl;
             if constexpr (F32) {
                 float y[8];
 #pragma unroll
-                for (int x = 0; x < 2; x++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) y[4 * x + e] = vf[x][e] == 0.0f ? 0.0f : vp[x].d[e][j] * vf[x][e];
+                for (int e = 0; e < 8; e++) y[e] = vf[e] == 0.0f ? 0.0f : vp[e / 4].d[e % 4][j] * vf[e];
                 split8(y, vh, vl);
             } else {
                 vh = codes8<FMT>(vp[0].d[j], vp[1].d[j]);
             }
 #pragma unroll
             for (int i = 0; i < QT; i++) {
-                const f16x8 hi = __builtin_bit_cast(f16x8, (u32x4){ph[i][0], ph[i][1], ph[i][2], ph[i][3]});
-                const f16x8 lo = __builtin_bit_cast(f16x8, (u32x4){pl[i][0], pl[i][1], pl[i][2], pl[i][3]});
-                o[i][j] = mfma(vh, lo, o[i][j]);
-                if constexpr (F32) o[i][j] = mfma(vl, hi, o[i][j]);
-                o[i][j] = mfma(vh, hi, o[i][j]);
+                o[i][j] = mfma(vh, lo[i], o[i][j]);
+                if constexpr (F32) o[i][j] = mfma(vl, hi[i], o[i][j]);
+                o[i][j] = mfma(vh, hi[i], o[i][j]);
             }
         }
     }
@@ -534,17 +543,16 @@ __global__ __launch_bounds__(512) void k_tree_attn(RowArgs a, KvLayer kv, TreeAt
 #pragma unroll
         for (int x = 0; x < 2; x++) vp[x].load(kv, block(0, x), s.h, lane);
         for (int c = 0; c < np; c++) {
-            const int p0 = it.page0 + 2 * (share + a.pw * (c0 + c));  // the pair's first page
             const int next = min(c + 1, np - 1);
-            float raw[2][QT][4];
-#pragma unroll
-            for (int x = 0; x < 2; x++) s.scores(kp[x], raw[x], lane);
+            float raw[QT][8], vsc[8], vf[8];
+            s.scores(kp, raw, lane);
 #pragma unroll
             for (int x = 0; x < 2; x++) kp[x].load(kv, block(next, x), s.h, lane);
-            if (s.masked(p0))
 #pragma unroll
-                for (int x = 0; x < 2; x++) s.mask(a, it, p0 + x, raw[x], lane);
-            s.gather(raw, vp);
+            for (int x = 0; x < 2; x++) value_scales<HD, FMT>(vp[x], &vsc[4 * x], &vf[4 * x]);
+            f16x8 hi[QT], lo[QT];
+            s.weights(a, it, it.page0 + 2 * (share + a.pw * (c0 + c)), raw, vsc, hi, lo, lane);
+            s.gather(hi, lo, vp, vf);
 #pragma unroll
             for (int x = 0; x < 2; x++) vp[x].load(kv, block(next, x), s.h, lane);
         }
@@ -562,8 +570,10 @@ __global__ __launch_bounds__(512) void k_tree_attn(RowArgs a, KvLayer kv, TreeAt
 template <int HD, int FMT, int RW>
 __global__ __launch_bounds__(512) void k_tree_attn_lds(RowArgs a, KvLayer kv, TreeAttn t) {
     constexpr int QT = 2, PW = RW == 2 ? 4 : 2, W = RW * PW, CPR = HD / 64;  // CPR: 16-byte chunks a lane takes of a page
-    constexpr int REC = 32 * HD + 128, STAGE = 2 * PW * REC, NST = RW == 2 ? 4 : 7;
-    constexpr int COPIES = (2 * PW * 2 * CPR + W - 1) / W;  // 1 KB copies a wave makes of a stage's codes
+    constexpr int SP = 2, PPS = 2 * SP * PW;  // pairs a share takes of a stage; pages of a stage
+    constexpr int REC = 32 * HD + 128, STAGE = PPS * REC, NST = RW == 2 ? 2 : 4;
+    constexpr int COPIES = (PPS * 2 * CPR + W - 1) / W;  // 1 KB copies a wave makes of a stage's codes
+    constexpr int SCOPIES = (PPS + W - 1) / W;             // and copies of a page's scales
     constexpr int JOIN = PW / 2 * RW * Slot<HD, FMT, QT>::ND * 64 * 4;
     static_assert(HD == 64 || HD == 128, "whole chunks");
     static_assert(W <= 8 && NST * STAGE + 4 * kPartPages <= 160 * 1024 && JOIN <= NST * STAGE, "a CU's LDS");
@@ -574,7 +584,7 @@ __global__ __launch_bounds__(512) void k_tree_attn_lds(RowArgs a, KvLayer kv, Tr
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int slot = wave % RW, share = wave / RW;
-    const int pages = it.page1 - it.page0, stages = (pages + 2 * PW - 1) / (2 * PW);
+    const int pages = it.page1 - it.page0, stages = (pages + PPS - 1) / PPS;
     for (int i = threadIdx.x; i < pages; i += 64 * W) ids[i] = a.btab[it.btab + it.page0 + i];
     Slot<HD, FMT, QT> s;
     s.start(a, t, it, kv.nkv, blockIdx.x % kv.nkv, slot, lane);
@@ -585,62 +595,84 @@ __global__ __launch_bounds__(512) void k_tree_attn_lds(RowArgs a, KvLayer kv, Tr
     int page[COPIES], to[COPIES];
 #pragma unroll
     for (int i = 0; i < COPIES; i++) {
-        const int q = min(wave + W * i, 2 * PW * 2 * CPR - 1), part = q % (2 * CPR), c = (part % CPR * 64 + lane) / 16;
+        const int q = min(wave + W * i, PPS * 2 * CPR - 1), part = q % (2 * CPR), c = (part % CPR * 64 + lane) / 16;
         page[i] = q / (2 * CPR);
         to[i] = page[i] * REC + part * 1024;
         off[i] = part < CPR ? r * HD + c * 16 : 16 * HD + c / CPR * (4 * HD) + r * (HD / 4) + c % CPR * 16;
     }
-    const int spage = wave % (2 * PW);  // and the scales of a page
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)ring;
-    auto record = [&](int stage, int pg) {  // past the last page the last again
-        const uint32_t id = __builtin_amdgcn_readfirstlane(ids[min(stage * 2 * PW + pg, pages - 1)]);
-        return kv.data + ((size_t)id * kv.nkv + s.h) * REC;
-    };
+    int held = 0, first = -64;  // a lane's block id, of 64 pages from `first` on
     auto copy = [&](int stage) {
         const uint32_t at = lds0 + stage % NST * STAGE;
-#pragma unroll
-        for (int i = 0; i < COPIES; i++) copy_to_lds(at + to[i], record(stage, page[i]), off[i]);
-        if (lane < 8) copy_to_lds(at + spage * REC + 32 * HD, record(stage, spage) + 32 * HD, 16 * lane);
-    };
-    for (int i = 0; i < NST - 1; i++) copy(i);
-    for (int st = 0; st < stages; st++) {
-        // this wave's copies of the stage have landed, then everyone's; and everyone has left the stage that the next
-        // copies overwrite
-        asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NST - 2) * (COPIES + 1)) : "memory");
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-        copy(st + NST - 1);
-        const int p0 = it.page0 + 2 * (share + PW * st);
-        if (!s.on || p0 >= s.last) continue;
-        const uint8_t* base = ring + st % NST * STAGE + 2 * share * REC;
-        float raw[2][QT][4];
-#pragma unroll
-        for (int x = 0; x < 2; x++) {
-            KeyPage<HD, FMT> k;
-#pragma unroll
-            for (int j = 0; j < CPR; j++) {
-                const u32x4 y = *(const u32x4*)(base + x * REC + ((g * CPR + j) * 16 + r) * 16);
-#pragma unroll
-                for (int e = 0; e < 4; e++) k.d[4 * j + e] = y[e];
-            }
-            k.s = *(const float4*)(base + x * REC + 32 * HD + 16 * g);
-            s.scores(k, raw[x], lane);
+        const int p0 = stage * PPS;
+        if (p0 >= first + 64) {
+            first = p0;
+            held = ids[min(p0 + lane, pages - 1)];  // past the last page the last again
         }
-        if (s.masked(p0))
+        auto record = [&](int pg) {
+            const uint32_t id = (uint32_t)__builtin_amdgcn_readlane(held, p0 - first + pg);
+            return kv.data + ((size_t)id * kv.nkv + s.h) * REC;
+        };
 #pragma unroll
-            for (int x = 0; x < 2; x++) s.mask(a, it, p0 + x, raw[x], lane);
-        ValuePage<HD, FMT> v[2];
+        for (int i = 0; i < COPIES; i++) copy_to_lds(at + to[i], record(page[i]), off[i]);
+#pragma unroll
+        for (int i = 0; i < SCOPIES; i++) {
+            const int pg = (wave + W * i) % PPS;
+            if (lane < 8) copy_to_lds(at + pg * REC + 32 * HD, record(pg) + 32 * HD, 16 * lane);
+        }
+    };
+    // a pair's record in the ring: pair u of the share's
+    auto pair = [&](int u) { return ring + u / SP % NST * STAGE + ((u % SP * PW + share) * 2) * REC; };
+    auto keys = [&](int u, KeyPage<HD, FMT> (&k)[2]) {
 #pragma unroll
         for (int x = 0; x < 2; x++) {
+            const uint8_t* base = pair(u) + x * REC;
 #pragma unroll
             for (int j = 0; j < CPR; j++) {
-                const u32x4 y = *(const u32x4*)(base + x * REC + 16 * HD + ((g * CPR + j) * 16 + r) * 16);
+                const u32x4 y = *(const u32x4*)(base + ((g * CPR + j) * 16 + r) * 16);
+#pragma unroll
+                for (int e = 0; e < 4; e++) k[x].d[4 * j + e] = y[e];
+            }
+            k[x].s = *(const float4*)(base + 32 * HD + 16 * g);
+        }
+    };
+    auto values = [&](int u, ValuePage<HD, FMT> (&v)[2], float (&sc)[8]) {
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+            const uint8_t* base = pair(u) + x * REC;
+            const float4 z = *(const float4*)(base + 32 * HD + 64 + 16 * g);
+            sc[4 * x] = z.x, sc[4 * x + 1] = z.y, sc[4 * x + 2] = z.z, sc[4 * x + 3] = z.w;
+#pragma unroll
+            for (int j = 0; j < CPR; j++) {
+                const u32x4 y = *(const u32x4*)(base + 16 * HD + ((g * CPR + j) * 16 + r) * 16);
 #pragma unroll
                 for (int e = 0; e < 4; e++) v[x].d[4 * j + e] = y[e];
             }
-            v[x].s = *(const float4*)(base + x * REC + 32 * HD + 64 + 16 * g);
         }
-        s.gather(raw, v);
+    };
+    for (int i = 0; i < NST - 1; i++) copy(i);
+    for (int st = 0; st < stages; st++) {
+        // this wave's copies of the stage have landed, then everyone's; and everyone is past the stage before
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NST - 2) * (COPIES + SCOPIES)) : "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        copy(st + NST - 1);  // over that one
+        const float none[8] = {};
+        KeyPage<HD, FMT> kp[2];
+        keys(st * SP, kp);
+#pragma unroll
+        for (int i = 0; i < SP; i++) {
+            const int u = st * SP + i, p0 = it.page0 + st * PPS + 2 * (i * PW + share);
+            if (!s.on || p0 >= s.last) break;
+            float raw[QT][8], vsc[8];
+            ValuePage<HD, FMT> vp[2];
+            f16x8 hi[QT], lo[QT];
+            s.scores(kp, raw, lane);
+            values(u, vp, vsc);  // on their way behind the weights
+            s.weights(a, it, p0, raw, vsc, hi, lo, lane);
+            if (i + 1 < SP) keys(u + 1, kp);
+            s.gather(hi, lo, vp, none);
+        }
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no copy is left on its way when the ring is reused, or given up
     __syncthreads();
