@@ -331,6 +331,7 @@ struct Slot {
         for (int x = 0; x < 2; x++)
 #pragma unroll
             for (int i = 0; i < QT; i++) acc[x][i] = (f32x4){0, 0, 0, 0};
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int s = 0; s < NS; s++) {
 #pragma unroll
@@ -348,6 +349,7 @@ struct Slot {
 #pragma unroll
                 for (int i = 0; i < QT; i++) acc[x][i] = mfma(k[x].hi[s], qh[i][s], acc[x][i]);
         }
+        __builtin_amdgcn_s_setprio(0);
 #pragma unroll
         for (int x = 0; x < 2; x++)
 #pragma unroll
@@ -420,6 +422,7 @@ struct Slot {
     // Adds a pair's weighted values; vf: value_scales' factors.
     __device__ __forceinline__ void gather(const f16x8 (&hi)[QT], const f16x8 (&lo)[QT], const ValuePage<HD, FMT> (&vp)[2],
                                            const float (&vf)[8]) {
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int j = 0; j < KD; j++) {
             f16x8 vh, vl;
@@ -438,6 +441,7 @@ struct Slot {
                 o[i][j] = mfma(vh, hi[i], o[i][j]);
             }
         }
+        __builtin_amdgcn_s_setprio(0);
     }
 
     // The sums of the pw position shares into share 0's, halving; a tile at a time, for the LDS that takes. Every
@@ -570,8 +574,8 @@ __global__ __launch_bounds__(512) void k_tree_attn(RowArgs a, KvLayer kv, TreeAt
 template <int HD, int FMT, int RW>
 __global__ __launch_bounds__(512) void k_tree_attn_lds(RowArgs a, KvLayer kv, TreeAttn t) {
     constexpr int QT = 2, PW = RW == 2 ? 4 : 2, W = RW * PW, CPR = HD / 64;  // CPR: 16-byte chunks a lane takes of a page
-    constexpr int SP = 2, PPS = 2 * SP * PW;  // pairs a share takes of a stage; pages of a stage
-    constexpr int REC = 32 * HD + 128, STAGE = PPS * REC, NST = RW == 2 ? 2 : 4;
+    constexpr int SP = RW == 2 ? 1 : 2, PPS = 2 * SP * PW;  // pairs a share takes of a stage; pages of a stage
+    constexpr int REC = 32 * HD + 128, STAGE = PPS * REC, NST = 4;
     constexpr int COPIES = (PPS * 2 * CPR + W - 1) / W;  // 1 KB copies a wave makes of a stage's codes
     constexpr int SCOPIES = (PPS + W - 1) / W;             // and copies of a page's scales
     constexpr int JOIN = PW / 2 * RW * Slot<HD, FMT, QT>::ND * 64 * 4;
@@ -651,29 +655,35 @@ __global__ __launch_bounds__(512) void k_tree_attn_lds(RowArgs a, KvLayer kv, Tr
         }
     };
     for (int i = 0; i < NST - 1; i++) copy(i);
+    // This wave's copies of all stages but the last `left` have landed, then everyone's.
+#define LANDED(left)                                                                               \
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((left) * (COPIES + SCOPIES)) : "memory");              \
+    __builtin_amdgcn_s_barrier();                                                                  \
+    asm volatile("" ::: "memory")
+    KeyPage<HD, FMT> kp[2];
+    LANDED(NST - 2);
+    keys(0, kp);
     for (int st = 0; st < stages; st++) {
-        // this wave's copies of the stage have landed, then everyone's; and everyone is past the stage before
-        asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NST - 2) * (COPIES + SCOPIES)) : "memory");
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-        copy(st + NST - 1);  // over that one
+        // the next stage is there too, for the keys that are read ahead, and everyone is past the stage before
+        LANDED(NST - 3);
         const float none[8] = {};
-        KeyPage<HD, FMT> kp[2];
-        keys(st * SP, kp);
 #pragma unroll
         for (int i = 0; i < SP; i++) {
             const int u = st * SP + i, p0 = it.page0 + st * PPS + 2 * (i * PW + share);
-            if (!s.on || p0 >= s.last) break;
+            const bool mine = s.on && p0 < s.last;
             float raw[QT][8], vsc[8];
             ValuePage<HD, FMT> vp[2];
             f16x8 hi[QT], lo[QT];
-            s.scores(kp, raw, lane);
+            if (mine) s.scores(kp, raw, lane);
+            if (i == 0) copy(st + NST - 1);  // over the stage before, its scalar work behind the products
+            if (!mine) continue;
             values(u, vp, vsc);  // on their way behind the weights
             s.weights(a, it, p0, raw, vsc, hi, lo, lane);
-            if (i + 1 < SP) keys(u + 1, kp);
+            keys(u + 1, kp);  // behind the values' products
             s.gather(hi, lo, vp, none);
         }
     }
+#undef LANDED
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no copy is left on its way when the ring is reused, or given up
     __syncthreads();
     s.join((float*)ring, slot, share, RW, PW, lane);
