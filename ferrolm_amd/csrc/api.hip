@@ -316,8 +316,8 @@ struct fg_rows {
     int heads = 1, kv_heads = 1, head_dim = 64, kv_blocks = 0;  // kv_blocks 0: no cache
     RowPlan plan;
     bool ready = false;
-    void *hmeta = nullptr, *dmeta = nullptr, *part = nullptr;
-    size_t hmeta_cap = 0, dmeta_cap = 0, part_cap = 0;
+    void *hmeta = nullptr, *dmeta = nullptr, *part = nullptr, *tree = nullptr;
+    size_t hmeta_cap = 0, dmeta_cap = 0, part_cap = 0, tree_cap = 0;
     hipEvent_t sent = nullptr;  // the plan's copy to the device
     RowArgs args() const { return row_args(plan, (const int32_t*)dmeta); }
 };
@@ -2518,6 +2518,9 @@ static int rows_plan(fg_rows* r, const fg_tree_seq* seqs, int32_t n_seqs) {
                                 (size_t)P.n_wi * r->kv_heads * attn_qmax(r->head_dim) * (r->head_dim + 4) * 4,
                                 r->ctx->stream, false)))
         return rc;
+    if (P.rooted && P.most_rows > kVerifyLdsRows &&
+        (rc = ensure(&r->tree, &r->tree_cap, ((size_t)kVerifyWords * P.rows + P.n_seqs) * 4, r->ctx->stream, false)))
+        return rc;
     if (!r->sent) HIPCHK(hipEventCreateWithFlags(&r->sent, hipEventDisableTiming));
     pack_rows(P, (int32_t*)r->hmeta);
     HIPCHK(hipMemcpyAsync(r->dmeta, r->hmeta, P.words * 4, hipMemcpyHostToDevice, r->ctx->stream));
@@ -2569,6 +2572,7 @@ void fg_rows_destroy(fg_rows* r) {
     const DeviceScope on(r->device);  // the context may be gone already
     if (r->dmeta) (void)hipFree(r->dmeta);  // waits for queued work that uses it
     if (r->part) (void)hipFree(r->part);
+    if (r->tree) (void)hipFree(r->tree);
     if (r->hmeta) (void)hipHostFree(r->hmeta);
     if (r->sent) (void)hipEventDestroy(r->sent);
     delete r;
@@ -2690,6 +2694,7 @@ int fg_tree_verify(fg_ctx* ctx, const fg_rows* r, int32_t drafts, int32_t vocab,
     v.out_path = out_path_dev;
     v.out_count = out_count_dev;
     v.ld = ld;
+    v.tree = (int32_t*)r->tree;
     launch_tree_verify(ctx->stream, r->args(), v);
     HIPCHK(hipGetLastError());
     return 0;
@@ -2773,6 +2778,7 @@ int fg_tree_step(fg_ctx* ctx, const fg_model* m, fg_kv* kv, const fg_tree_seq* s
             for (int s = 0; s < n_seqs; s++) sampling |= params[s].temperature > 0.0f;
         }
         size_t rows = 0;
+        int most = 0;
         for (int s = 0; s < n_seqs; s++) {
             const fg_tree_seq& q = seqs[s];
             if (q.n <= 0) return fail(FG_E_ARG, "a tree has at least one row");
@@ -2787,10 +2793,12 @@ int fg_tree_step(fg_ctx* ctx, const fg_model* m, fg_kv* kv, const fg_tree_seq* s
             }
             if (ld < deepest) return fail(FG_E_SHAPE, "the outputs hold fewer tokens than the longest branch has rows");
             rows += q.n;
+            most = std::max(most, q.n);
         }
         // behind the plan: a parameter set and a uniform number per row, the outputs
         const size_t o_prm = 0, o_u = o_prm + rows * 4, o_out = (o_u + rows + 63) / 64 * 64, o_path = o_out + (size_t)n_seqs * ld,
-                     o_cnt = o_path + (size_t)n_seqs * ld, more = o_cnt + n_seqs;
+                     o_cnt = o_path + (size_t)n_seqs * ld, o_tree = o_cnt + n_seqs,
+                     more = o_tree + (most > kVerifyLdsRows ? kVerifyWords * rows + n_seqs : 0);
         Plan P;
         Work w{};
         rc = tree_forward(
@@ -2827,13 +2835,14 @@ int fg_tree_step(fg_ctx* ctx, const fg_model* m, fg_kv* kv, const fg_tree_seq* s
             v.out_path = dx + o_path;
             v.out_count = dx + o_cnt;
             v.ld = ld;
+            v.tree = (int32_t*)(dx + o_tree);
             launch_tree_verify(st, ra, v);
         } else {
             launch_tree_accept(st, ra, tokens, w.am, (uint32_t*)(dx + o_out), dx + o_path, dx + o_cnt, ld);
         }
         launch_kv_commit(st, ra, kv->layer(0), (int)m->layers.size(), kv->layer_bytes(), dx + o_path, dx + o_cnt, ld);
         HIPCHK(hipGetLastError());
-        HIPCHK(hipMemcpyAsync(hx + o_out, dx + o_out, (more - o_out) * 4, hipMemcpyDeviceToHost, st));
+        HIPCHK(hipMemcpyAsync(hx + o_out, dx + o_out, (o_tree - o_out) * 4, hipMemcpyDeviceToHost, st));
         HIPCHK(hipStreamSynchronize(st));
         memcpy(out_tokens, hx + o_out, (size_t)n_seqs * ld * 4);
         memcpy(out_path, hx + o_path, (size_t)n_seqs * ld * 4);

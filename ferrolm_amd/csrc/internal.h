@@ -384,7 +384,8 @@ struct RowArgs {
     const int32_t* rpos = nullptr;   // per row: its position on its branch
     const uint16_t* masks = nullptr; // per row of a tree and page from pos / 16 on: tokens that it sees
     const int32_t *cstart = nullptr, *clist = nullptr;  // children of each row, in order
-    int n_seqs = 0, rows = 0, n_items = 0, n_wi = 0, n_quads = 0, longest = 0, widest = 0;  // widest: most children of a row
+    const int32_t* parent = nullptr;                    // in the row's sequence, -1: none
+    int n_seqs = 0, rows = 0, n_items = 0, n_wi = 0, n_quads = 0, longest = 0, most_rows = 0;  // most_rows: of a sequence
     bool unused = false, parts = false;  // some row is unused; some row has several items
     int qt = 0, rw = 0, pw = 0;      // 16-query tiles a wave, row slots and position shares a workgroup
 };
@@ -417,11 +418,13 @@ int launch_tree_attn(hipStream_t st, const RowArgs& a, const KvLayer& kv, const 
 int launch_merge(hipStream_t st, const AttnArgs& a, int m, int consumer_kind, Pieces& out);
 
 enum { DRAFT_EACH = 0, DRAFT_DISTINCT = 1, DRAFT_FIXED = 2 };
+constexpr int kVerifyLdsRows = 1024, kVerifyWords = 7;  // rows of a tree that the walk holds in LDS; words of a row
 struct VerifyArgs {
     const uint32_t* tokens = nullptr;  // [row]
     const float *p = nullptr, *q = nullptr;  // [row][vocab]
     const float* u = nullptr;          // [row]: a first row's is its sequence's final draw, others' their test
     int vocab = 0, kind = 0;
+    int32_t* tree = nullptr;           // kVerifyWords per row and one per sequence, when most_rows > kVerifyLdsRows
     uint32_t* out_tokens = nullptr;    // [sequence][ld]
     int32_t* out_path = nullptr;
     int32_t* out_count = nullptr;      // [sequence]

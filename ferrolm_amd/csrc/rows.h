@@ -25,16 +25,16 @@ constexpr int kTreeRows = 4096;
 constexpr int tree_workgroups(int rw) { return rw > 1 ? 256 : 512; }
 
 struct RowPlan {
-    int n_seqs = 0, rows = 0, n_wi = 0, n_items = 0, n_quads = 0, longest = 0, deepest = 0, widest = 0;
+    int n_seqs = 0, rows = 0, n_wi = 0, n_items = 0, n_quads = 0, longest = 0, deepest = 0, most_rows = 0;
     uint32_t top_block = 0;  // the highest block id
     int64_t tokens = 0;  // cached tokens of all sequences, rows among them
     int qt = 1, rw = 1, pw = 1;
     bool unused = false, parts = false;  // some row is unused; some row has several items
     bool rooted = true;  // every sequence's rows hang on its first
-    std::vector<int32_t> seqs, btab, items, mrec, quads, rpos, cstart, clist;
+    std::vector<int32_t> seqs, btab, items, mrec, quads, rpos, cstart, clist, parent;
     std::vector<uint16_t> masks;
     size_t o_seqs = 0, o_btab = 0, o_items = 0, o_mrec = 0, o_quads = 0, o_rpos = 0, o_masks = 0, o_cstart = 0,
-           o_clist = 0, words = 0;
+           o_clist = 0, o_parent = 0, words = 0;
 };
 
 // Checked by the caller: n >= 0, parents[i] in [-2, i), a block for every position.
@@ -63,6 +63,7 @@ inline void plan_rows(RowPlan& P, const RowSeq* in, int n_seqs, int nh, int nkv,
         for (int i = 0; i < q.n; i++) {
             const int p = chain ? i - 1 : q.parents[i];
             depth[i] = p >= 0 ? depth[p] + 1 : 0;
+            P.parent.push_back(std::max(p, -1));
             if (p >= 0) kids[p + 1]++;
             P.rooted = P.rooted && (i == 0 ? p == -1 : p != -1);
             P.unused = P.unused || p == -2;
@@ -74,10 +75,8 @@ inline void plan_rows(RowPlan& P, const RowSeq* in, int n_seqs, int nh, int nkv,
             a[i / 64] |= 1ull << (i % 64);
         }
         P.rooted = P.rooted && q.n > 0;
-        for (int i = 0; i < q.n; i++) {
-            P.widest = std::max(P.widest, kids[i + 1]);
-            kids[i + 1] += kids[i];
-        }
+        P.most_rows = std::max(P.most_rows, q.n);
+        for (int i = 0; i < q.n; i++) kids[i + 1] += kids[i];
         const int c0 = (int)P.clist.size();
         for (int i = 0; i < q.n; i++) P.cstart.push_back(c0 + kids[i]);
         P.clist.resize(c0 + kids[q.n]);
@@ -197,6 +196,7 @@ inline void plan_rows(RowPlan& P, const RowSeq* in, int n_seqs, int nh, int nkv,
     P.o_masks = place((P.masks.size() + 1) / 2);
     P.o_cstart = place(P.cstart.size());
     P.o_clist = place(P.clist.size());
+    P.o_parent = place(P.parent.size());
 }
 
 inline void pack_rows(const RowPlan& P, int32_t* h) {
@@ -211,6 +211,7 @@ inline void pack_rows(const RowPlan& P, int32_t* h) {
     cp(P.o_rpos, P.rpos);
     cp(P.o_cstart, P.cstart);
     cp(P.o_clist, P.clist);
+    cp(P.o_parent, P.parent);
     if (!P.masks.empty()) std::memcpy(h + P.o_masks, P.masks.data(), P.masks.size() * 2);
 }
 
@@ -225,13 +226,14 @@ inline RowArgs row_args(const RowPlan& P, const int32_t* d) {
     a.masks = (const uint16_t*)(d + P.o_masks);
     a.cstart = d + P.o_cstart;
     a.clist = d + P.o_clist;
+    a.parent = d + P.o_parent;
     a.n_seqs = P.n_seqs;
     a.rows = P.rows;
     a.n_items = P.n_items;
     a.n_wi = P.n_wi;
     a.n_quads = P.n_quads;
     a.longest = P.longest;
-    a.widest = P.widest;
+    a.most_rows = P.most_rows;
     a.unused = P.unused;
     a.parts = P.parts;
     a.qt = P.qt;

@@ -25,41 +25,92 @@ constexpr int kVerifyThreads = 1024, kVerifyWaves = kVerifyThreads / 64;
 // What q's tokens drawn so far leave of its sum, below which it is spent: a sum of f32 probabilities is 1 only to
 // about that.
 constexpr double kSpent = 0x1p-20;
-constexpr int kKids = 256;  // children of a node taken at a time
 
 __device__ __forceinline__ double wave_sum(double x) {
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1) x += __shfl_xor(x, m);
     return x;
 }
+// x > 0, or 0: a NaN counts as 0
+__device__ __forceinline__ double mass_of(float x) { return x > 0.0f ? (double)x : 0.0; }
 
 // What is left of a node's distribution.
 struct Left {
     const float *p, *q;  // q: nullptr for given drafts
     double a;
-    const uint32_t* gone;  // given drafts: the tokens removed
-    int n_gone;
-    __device__ __forceinline__ double at(int t) const {
-        const float x = p[t];
-        const double w = x > 0.0f ? (double)x : 0.0;  // a NaN counts as 0
-        if (q) {
-            const float y = q[t];
-            const double r = w - a * (y > 0.0f ? (double)y : 0.0);
-            return r > 0.0 ? r : 0.0;
+    template <bool Q>
+    __device__ __forceinline__ double of(float x, float y) const {
+        return Q ? fmax(mass_of(x) - a * mass_of(y), 0.0) : mass_of(x);
+    }
+};
+// Given drafts: the tokens of the node's children, whose mass is removed.
+struct Gone {
+    const uint32_t* at;
+    int n;
+    // f(token) for those in [first, last), by whole waves
+    template <class F>
+    __device__ __forceinline__ void each(int first, int last, const F& f) const {
+        const int lane = threadIdx.x & 63;
+        for (int i = 0; i < n; i += 64) {
+            const uint32_t g = at[min(i + lane, n - 1)];
+            uint64_t in = __ballot(i + lane < n && g >= (uint32_t)first && g < (uint32_t)last);
+            for (; in; in &= in - 1) f((int)__builtin_amdgcn_readlane(g, __builtin_ctzll(in)));
         }
-        for (int i = 0; i < n_gone; i++)
-            if (gone[i] == (uint32_t)t) return 0.0;
-        return w;
     }
 };
 
-// Sums of 16 consecutive shares of [first, last), one a wave; every thread returns their total.
-__device__ __forceinline__ int share_len(int n) { return (n + kVerifyWaves - 1) / kVerifyWaves; }
-__device__ double shares(const Left& f, int first, int last, double* sums) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, len = share_len(last - first);
+// Sums of 16 consecutive shares of [first, last), one a wave, into sums; every thread returns their total. V4: rows
+// are 16-byte aligned and the shares whole groups of four.
+template <bool V4>
+__device__ __forceinline__ int share_len(int n) {
+    const int len = (n + kVerifyWaves - 1) / kVerifyWaves;
+    return V4 ? (len + 3) / 4 * 4 : len;
+}
+// A wave's share, UN loads of each row on their way per lane, of four values (V4) or one: they take no branch (past
+// the end they read the last again), so that none waits for another.
+template <bool V4, bool Q>
+__device__ __forceinline__ double share_sum(const Left& f, const Gone& gone, int t0, int t1) {
+    constexpr int UN = 8, E = V4 ? 4 : 1;
+    const int lane = threadIdx.x & 63;
+    double s[4] = {0.0, 0.0, 0.0, 0.0};
+    for (int b = t0; b < t1; b += UN * E * 64) {
+        float x[UN][E], y[UN][E];
+#pragma unroll
+        for (int k = 0; k < UN; k++) {
+            const int t = min(b + (k * 64 + lane) * E, t1 - E);
+            if constexpr (V4) {
+                const f32x4 pv = __builtin_nontemporal_load((const f32x4*)(f.p + t));
+                f32x4 qv = (f32x4){0, 0, 0, 0};
+                if (Q) qv = __builtin_nontemporal_load((const f32x4*)(f.q + t));
+#pragma unroll
+                for (int e = 0; e < 4; e++) x[k][e] = pv[e], y[k][e] = qv[e];
+            } else {
+                x[k][0] = __builtin_nontemporal_load(f.p + t);
+                y[k][0] = Q ? __builtin_nontemporal_load(f.q + t) : 0.0f;
+            }
+        }
+        if constexpr (!Q)
+            gone.each(b, b + UN * E * 64, [&](int g) {
+#pragma unroll
+                for (int k = 0; k < UN; k++)
+#pragma unroll
+                    for (int e = 0; e < E; e++) x[k][e] = b + (k * 64 + lane) * E + e == g ? 0.0f : x[k][e];
+            });
+#pragma unroll
+        for (int k = 0; k < UN; k++) {
+            const float in = b + (k * 64 + lane) * E < t1 ? 1.0f : 0.0f;  // a NaN stays one, and counts as 0
+#pragma unroll
+            for (int e = 0; e < E; e++) s[V4 ? e : k & 3] += f.of<Q>(x[k][e] * in, y[k][e]);
+        }
+    }
+    return (s[0] + s[1]) + (s[2] + s[3]);
+}
+template <bool V4>
+__device__ double shares(const Left& f, const Gone& gone, int first, int last, double* sums) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, len = share_len<V4>(last - first);
     const int t0 = first + wave * len, t1 = min(last, t0 + len);
     double x = 0.0;
-    for (int t = t0 + lane; t < t1; t += 64) x += f.at(t);
+    if (t0 < t1) x = f.q ? share_sum<V4, true>(f, gone, t0, t1) : share_sum<V4, false>(f, gone, t0, t1);
     x = wave_sum(x);
     __syncthreads();  // the sums of the call before have been read
     if (lane == 0) sums[wave] = x;
@@ -88,125 +139,173 @@ __device__ __forceinline__ int pick(const double* sums, double& target) {
     return last;
 }
 
+// A sequence's rows as the walk needs them: each row's children, and of each row its token, its probabilities at
+// its parent, its random number and whether an earlier sibling has its token.
+struct Tree {
+    int32_t *cstart, *clist;  // relative to the sequence
+    uint32_t* tok;
+    float *p, *q, *u;
+    int32_t* seen;
+    static constexpr int kWords = kVerifyWords;  // of a row, and one word more
+    __device__ Tree(int32_t* at, int n) {
+        cstart = at;
+        clist = cstart + n + 1;
+        tok = (uint32_t*)(clist + n);
+        p = (float*)(tok + n);
+        q = p + n;
+        u = q + n;
+        seen = (int32_t*)(u + n);
+    }
+};
+
 }  // namespace
 
-// One workgroup per sequence.
+// One workgroup per sequence. The walk itself reads nothing from memory: what it can ask for is gathered first, all
+// rows at once, into LDS (MEM: into v.tree, where some sequence has more than kVerifyLdsRows rows).
+template <bool V4, bool MEM>
 __global__ __launch_bounds__(kVerifyThreads) void k_tree_verify(RowArgs a, VerifyArgs v) {
     __shared__ double sums[kVerifyWaves];
-    __shared__ uint32_t ctok[kKids];
-    __shared__ float cp[kKids], cq[kKids], cu[kKids];
-    __shared__ int seen[kKids];  // an earlier sibling has the token
-    const int s = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
-    const int row0 = a.seqs[(size_t)s * kSeqWords], V = v.vocab;
+    extern __shared__ int32_t mem[];
+    const int s = blockIdx.x, tid = threadIdx.x, lane = tid & 63, V = v.vocab;
+    const int row0 = a.seqs[(size_t)s * kSeqWords], n = a.seqs[(size_t)s * kSeqWords + 1];
+    const Tree tr(MEM ? v.tree + (size_t)Tree::kWords * row0 + s : mem, n);
     uint32_t* out = v.out_tokens + (size_t)s * v.ld;
     int32_t* path = v.out_path + (size_t)s * v.ld;
-    int node = row0, count = 1, known = 0;  // known: sums holds the shares of what is left
+    const int c0 = a.cstart[row0];
+    for (int i = tid; i <= n; i += kVerifyThreads) tr.cstart[i] = a.cstart[row0 + i] - c0;
+    for (int i = tid; i < n; i += kVerifyThreads) {
+        const uint32_t t = v.tokens[row0 + i];
+        const int parent = a.parent[row0 + i];  // -1 for a first or unused row
+        const bool in = parent >= 0 && t < (uint32_t)V;  // a token outside the vocabulary never passes
+        const size_t at = in ? (size_t)(row0 + parent) * V + t : 0;
+        tr.tok[i] = t;
+        tr.u[i] = v.u[row0 + i];
+        tr.p[i] = in ? v.p[at] : 0.0f;
+        tr.q[i] = in ? (v.kind == DRAFT_FIXED ? 1.0f : v.q[at]) : 0.0f;
+        tr.seen[i] = 0;
+    }
+    __syncthreads();
+    for (int i = tid; i < tr.cstart[n]; i += kVerifyThreads) tr.clist[i] = a.clist[c0 + i] - row0;
+    __syncthreads();
+    if (v.kind != DRAFT_EACH) {
+        for (int i = tid; i < n; i += kVerifyThreads)
+            for (int j = tr.cstart[i] + 1; j < tr.cstart[i + 1]; j++)
+                for (int k = tr.cstart[i]; k < j; k++)
+                    if (tr.tok[tr.clist[k]] == tr.tok[tr.clist[j]]) tr.seen[tr.clist[j]] = 1;
+        __syncthreads();
+    }
+    int node = 0, count = 1;
+    bool known = false;  // sums holds the shares of what is left
     Left left{};
+    Gone gone{};
     double total = 0.0;
     if (tid == 0) path[0] = 0;
     for (;;) {
-        const int c0 = a.cstart[node], nc = a.cstart[node + 1] - c0;
-        left = Left{v.p + (size_t)node * V, v.kind == DRAFT_FIXED ? nullptr : v.q + (size_t)node * V, 0.0, nullptr, 0};
-        known = 0;
+        const size_t row = (size_t)(row0 + node) * V;
+        left = Left{v.p + row, v.kind == DRAFT_FIXED ? nullptr : v.q + row, 0.0};
+        known = false;
         double b = 1.0, d = 1.0;
         int passed = -1;
-        for (int j0 = 0; j0 < nc && passed < 0 && b > 0.0; j0 += kKids) {
-            const int m = min(kKids, nc - j0);
-            __syncthreads();
-            for (int j = tid; j < m; j += kVerifyThreads) {
-                const int row = a.clist[c0 + j0 + j];
-                const uint32_t t = v.tokens[row];
-                const bool in = t < (uint32_t)V;  // a token outside the vocabulary never passes
-                const float x = in ? left.p[t] : 0.0f, y = in ? (left.q ? left.q[t] : 1.0f) : 0.0f;
-                ctok[j] = t;
-                cu[j] = v.u[row];
-                cp[j] = x > 0.0f ? x : 0.0f;
-                cq[j] = y > 0.0f ? y : 0.0f;
-                int before = 0;
-                if (v.kind != DRAFT_EACH)
-                    for (int i = 0; i < j0 + j && !before; i++) before = v.tokens[a.clist[c0 + i]] == t;
-                seen[j] = before;
+        for (int j = tr.cstart[node]; j < tr.cstart[node + 1] && passed < 0; j++) {
+            const int c = tr.clist[j];
+            const bool seen = tr.seen[c];
+            const double p = mass_of(tr.p[c]), q = mass_of(tr.q[c]), u = tr.u[c];
+            double mass, rate;
+            if (v.kind == DRAFT_FIXED) {
+                mass = seen ? 0.0 : p / b;
+                rate = q;
+            } else {
+                // without replacement: a token drawn before, or one that q had nothing left for, was not drawn
+                if (v.kind == DRAFT_DISTINCT && (seen || d < kSpent || q == 0.0)) continue;
+                const double r = p - left.a * q;
+                rate = q / d;
+                mass = (r > 0.0 ? r : 0.0) / b;
             }
-            __syncthreads();
-            for (int j = 0; j < m; j++) {
-                const double p = cp[j], q = cq[j], u = cu[j];
-                double mass, rate;
-                if (v.kind == DRAFT_FIXED) {
-                    mass = seen[j] ? 0.0 : p / b;
-                    rate = q;
-                } else {
-                    // without replacement: a token drawn before, or one that q had nothing left for, was not drawn
-                    if (v.kind == DRAFT_DISTINCT && (seen[j] || d < kSpent || q == 0.0)) continue;
-                    const double r = p - left.a * q;
-                    rate = q / d;
-                    mass = (r > 0.0 ? r : 0.0) / b;
-                }
-                if (u * rate < mass && rate > 0.0) {
-                    passed = a.clist[c0 + j0 + j];
-                    break;
-                }
-                if (v.kind == DRAFT_FIXED) {
-                    if (!seen[j]) b -= p;
-                } else {
-                    left.a += b / d;
-                    if (v.kind == DRAFT_DISTINCT) d -= q;
-                    b = total = shares(left, 0, V, sums);
-                    known = 1;
-                    if (!(b > 0.0)) break;  // nothing is left: no child passes
-                }
+            if (u * rate < mass && rate > 0.0) {
+                passed = c;
+            } else if (v.kind == DRAFT_FIXED) {
+                if (!seen) b -= p;
+            } else {
+                left.a += b / d;
+                if (v.kind == DRAFT_DISTINCT) d -= q;
+                b = total = shares<V4>(left, gone, 0, V, sums);
+                known = true;
+                if (!(b > 0.0)) break;  // nothing is left: no child passes
             }
         }
-        if (passed < 0) {
-            if (v.kind == DRAFT_FIXED && nc > 0) left.n_gone = nc;
-            break;
-        }
+        if (passed < 0) break;
         if (tid == 0) {
-            out[count - 1] = v.tokens[passed];
-            path[count] = passed - row0;
+            out[count - 1] = tr.tok[passed];
+            path[count] = passed;
         }
         node = passed;
         count++;
     }
-    // the removed tokens of a node with given drafts
-    __shared__ uint32_t gone[kKids];
-    extern __shared__ uint32_t more[];
-    if (left.n_gone) {
-        uint32_t* g = left.n_gone <= kKids ? gone : more;
-        for (int i = tid; i < left.n_gone; i += kVerifyThreads) g[i] = v.tokens[a.clist[a.cstart[node] + i]];
-        left.gone = g;
+    if (v.kind == DRAFT_FIXED && tr.cstart[node + 1] > tr.cstart[node]) {
+        // the removed tokens, over the probabilities, which have been used
+        __syncthreads();
+        uint32_t* g = (uint32_t*)tr.p;
+        gone = Gone{g, tr.cstart[node + 1] - tr.cstart[node]};
+        for (int i = tid; i < gone.n; i += kVerifyThreads) g[i] = tr.tok[tr.clist[tr.cstart[node] + i]];
         __syncthreads();
     }
-    if (!known) total = shares(left, 0, V, sums);
+    if (!known) total = shares<V4>(left, gone, 0, V, sums);
     if (!(total > 0.0)) {  // nothing is left: the target's own distribution
         left.a = 0.0;
         left.q = nullptr;
-        left.n_gone = 0;
-        total = shares(left, 0, V, sums);
+        gone.n = 0;
+        total = shares<V4>(left, gone, 0, V, sums);
     }
-    double target = (double)v.u[row0] * total;
+    double target = (double)tr.u[0] * total;
     int first = 0, last = V;
     for (int round = 0; round < 2; round++) {
-        if (round) (void)shares(left, first, last, sums);
-        const int w = pick(sums, target), len = share_len(last - first);
+        if (round) (void)shares<V4>(left, gone, first, last, sums);
+        const int w = pick(sums, target), len = share_len<V4>(last - first);
         first += w * len;
         last = max(first, min(last, first + len));
     }
     if (tid >= 64) return;
-    // one wave, in token order
+    // one wave, in token order: a lane's consecutive tokens, eight at a time
     int found = -1, positive = 0;
     double c = 0.0;
-    for (int t0 = first; t0 < last && found < 0; t0 += 64) {
-        const int t = t0 + lane;
-        const double w = t < last ? left.at(t) : 0.0;
-        double x = w;
+    for (int t0 = first; t0 < last && found < 0; t0 += 512) {
+        double w[8], mine = 0.0;
+        float px[8], qx[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const int t = min(t0 + 8 * lane + e, last - 1);
+            px[e] = left.p[t];
+            qx[e] = left.q ? left.q[t] : 0.0f;
+        }
+        gone.each(t0, t0 + 512, [&](int g) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) px[e] = t0 + 8 * lane + e == g ? 0.0f : px[e];
+        });
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const double x = left.q ? left.of<true>(px[e], qx[e]) : left.of<false>(px[e], 0.0f);
+            w[e] = t0 + 8 * lane + e < last ? x : 0.0;
+            mine += w[e];
+        }
+        double x = mine;
 #pragma unroll
         for (int m = 1; m < 64; m <<= 1) {
             const double y = __shfl_up(x, m);
             if (lane >= m) x += y;
         }
-        const uint64_t any = __ballot(w > 0.0), hit = __ballot(c + x > target && w > 0.0);
-        if (hit) found = t0 + __builtin_ctzll(hit);
-        if (any) positive = t0 + 63 - __builtin_clzll(any);
+        double run = c + (x - mine);
+        int hit = -1, top = -1;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            run += w[e];
+            if (w[e] > 0.0) {
+                top = t0 + 8 * lane + e;
+                if (hit < 0 && run > target) hit = top;
+            }
+        }
+        const uint64_t hits = __ballot(hit >= 0), tops = __ballot(top >= 0);
+        if (tops) positive = __shfl(top, 63 - __builtin_clzll(tops));
+        if (hits) found = __shfl(hit, __builtin_ctzll(hits));
         c += __shfl(x, 63);
     }
     if (lane == 0) {
@@ -219,10 +318,24 @@ __global__ __launch_bounds__(kVerifyThreads) void k_tree_verify(RowArgs a, Verif
     }
 }
 
-void launch_tree_verify(hipStream_t st, const RowArgs& a, const VerifyArgs& v) {
+void launch_tree_verify(hipStream_t st, const RowArgs& a, const VerifyArgs& v0) {
     if (a.n_seqs <= 0) return;
-    const size_t more = v.kind == DRAFT_FIXED && a.widest > kKids ? (size_t)a.widest * 4 : 0;
-    hipLaunchKernelGGL(k_tree_verify, dim3(a.n_seqs), dim3(kVerifyThreads), more, st, a, v);
+    const VerifyArgs v = v0;
+    const size_t lds = (size_t)(Tree::kWords * a.most_rows + 1) * 4;
+    const bool v4 = v.vocab % 4 == 0 && ((uintptr_t)v.p | (uintptr_t)v.q) % 16 == 0;
+    auto go = [&](auto k, size_t bytes) {
+        hipLaunchKernelGGL(k, dim3(a.n_seqs), dim3(kVerifyThreads), bytes, st, a, v);
+    };
+    if (a.most_rows > kVerifyLdsRows) {
+        if (v4)
+            go(k_tree_verify<true, true>, 0);
+        else
+            go(k_tree_verify<false, true>, 0);
+    } else if (v4) {
+        go(k_tree_verify<true, false>, lds);
+    } else {
+        go(k_tree_verify<false, false>, lds);
+    }
 }
 
 // One wave per sequence.

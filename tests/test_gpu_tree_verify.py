@@ -222,3 +222,17 @@ def test_greedy_walk(ctx):
             assert count[s] == k and out[s, :k].tolist() == want and path[s, :k].tolist() == way
             assert not out[s, k:].any() and (path[s, k:] == -1).all()
             at += len(parents)
+
+
+@pytest.mark.parametrize("drafts", gpu.DRAFTS)
+def test_trees_that_leave_the_lds(ctx, drafts):
+    """More rows than a workgroup holds, beside a small tree; a chain of as many."""
+    rng = np.random.default_rng(12)
+    big = [-1] + [int(x) for x in rng.integers(0, np.arange(1, 1500) // 8 + 1)]
+    for tree in (big, list(range(-1, 1200))):
+        seqs = [TREES[3], tree, TREES[1]]
+        rows = sum(map(len, seqs))
+        p, q = distributions(rng, rows, 301, peak=1.0, noise=0.5)
+        tokens = drafted(rng, seqs, q, drafts)
+        for _ in range(3):
+            check(ctx, seqs, tokens, p, None if drafts == "fixed" else q, rng.random(rows, np.float32), drafts)
