@@ -373,8 +373,9 @@ struct KvLayer {  // one layer of a cache
 // Device arrays of a set of rows (RowPlan in rows.h lays them out).
 constexpr int kSeqWords = 8;   // first row, rows, pos, first block in btab, first mask word (-1: a chain),
                                // mask words per row, first token of the read-back, tokens cached
-constexpr int kItemWords = 8;  // sequence (-1: unused), first row, first and last page, first partial slot, slots
-                               // between the item's row slots, row slots, 1: no other item has these rows
+constexpr int kItemWords = 16; // sequence (-1: unused), first row, first and last page, first partial slot, slots
+                               // between the item's row slots, row slots, 1: no other item has these rows; the
+                               // first six words of the sequence
 constexpr int kPartPages = 1024; // most pages of an item
 struct RowArgs {
     const int32_t *seqs = nullptr, *btab = nullptr, *items = nullptr;

@@ -20,9 +20,11 @@ struct RowSeq {
 
 // Longest tree: its masks hold a bit per row and token of the tree.
 constexpr int kTreeRows = 4096;
-// Workgroups that an attention launch is cut into at most, where it has not more row groups: what the card
-// runs at a time, one workgroup a CU of several slots, two of one.
-constexpr int tree_workgroups(int rw) { return rw > 1 ? 256 : 512; }
+// Workgroups that an attention launch is cut into at most, where it has not more row groups: one a CU. More cost more
+// in the merge than they gain: us of a tree over a long fp8 context in 256, 384, 512 workgroups 149, 196, 170,
+// of trees of 16 sequences 70, 82, 79; one token over 32000 fp8 tokens (8 heads, workgroups of four waves) in
+// 256, 512, 1024 21.9, 23.6, 33.4, eight chains of 5 17.5, 19.6, 25.0, one token of 16 sequences 22.7, 20.9, 24.9.
+constexpr int kTreeWorkgroups = 256;
 
 struct RowPlan {
     int n_seqs = 0, rows = 0, n_wi = 0, n_items = 0, n_quads = 0, longest = 0, deepest = 0, most_rows = 0;
@@ -119,7 +121,7 @@ inline void plan_rows(RowPlan& P, const RowSeq* in, int n_seqs, int nh, int nkv,
     P.cstart.push_back((int32_t)P.clist.size());
     P.qt = most_q <= 16 ? 1 : qm / 16;
     P.rw = std::min(4, most_slots);
-    P.pw = P.rw == 1 ? 8 : P.rw == 2 ? 4 : 2;
+    P.pw = P.rw <= 2 ? 4 : 2;
     // items: rw slots of rows x a part of the pages that they see, in parts of even length
     auto group_pages = [&](const RowSeq& q, int r0) {
         const bool chain = P.seqs[(&q - in) * kSeqWords + 4] < 0;
@@ -135,7 +137,7 @@ inline void plan_rows(RowPlan& P, const RowSeq* in, int n_seqs, int nh, int nkv,
     auto fits = [&](int len) {
         int64_t n = 0;
         for (int pages : groups) n += parts_of(pages, len);
-        return n * nkv <= tree_workgroups(P.rw);
+        return n * nkv <= kTreeWorkgroups;
     };
     int lo = 1, hi = kPartPages / step;  // in rounds
     while (lo < hi) {
@@ -153,8 +155,9 @@ inline void plan_rows(RowPlan& P, const RowSeq* in, int n_seqs, int nh, int nkv,
             const int per = ((pages + parts - 1) / parts + step - 1) / step * step;
             const int np = parts_of(pages, per), slots = std::min(P.rw, (q.n - r0 + rps - 1) / rps);
             for (int p = 0; p < np; p++) {
+                const int32_t* sr = &P.seqs[(size_t)s * kSeqWords];
                 const int32_t rec[kItemWords] = {s, r0, p * per, std::min(pages, (p + 1) * per), P.n_wi + p, np, slots,
-                                                 np == 1};
+                                                 np == 1, sr[0], sr[1], sr[2], sr[3], sr[4], sr[5], 0, 0};
                 P.items.insert(P.items.end(), rec, rec + kItemWords);
                 P.n_items++;
             }

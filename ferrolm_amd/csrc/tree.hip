@@ -239,11 +239,9 @@ struct Item {
     int row0, page0, page1, wi, wi_step, slots, alone;
     bool chain;
     __device__ __forceinline__ bool read(const RowArgs& a, int item) {
-        const int4 i0 = *(const int4*)(a.items + (size_t)item * kItemWords),
-                   i1 = *(const int4*)(a.items + (size_t)item * kItemWords + 4);
+        const int4* p = (const int4*)(a.items + (size_t)item * kItemWords);
+        const int4 i0 = p[0], i1 = p[1], s0 = p[2], s1 = p[3];
         if (i0.x < 0) return false;  // an unused item of the launch's capacity
-        const int32_t* s = a.seqs + (size_t)i0.x * kSeqWords;
-        const int4 s0 = *(const int4*)s, s1 = *(const int4*)(s + 4);
         seq0 = s0.x, n = s0.y, pos = s0.z, btab = s0.w, mask0 = s1.x, mpages = s1.y;
         chain = mask0 < 0;
         row0 = i0.y, page0 = i0.z, page1 = i0.w, wi = i1.x, wi_step = i1.y, slots = i1.z, alone = i1.w;
@@ -264,8 +262,7 @@ struct Slot {
     int h, G, r0, nr, last, full;  // first row and rows; pages that they see; tokens that all of them see
     bool on;
 
-    __device__ __forceinline__ void start(const RowArgs& a, const TreeAttn& t, const Item& it, int nkv, int head, int slot,
-                                          int lane) {
+    __device__ __forceinline__ void place(const TreeAttn& t, const Item& it, int nkv, int head, int slot) {
         h = head;
         G = t.nh / nkv;
         r0 = it.row0 + slot * (QM / G);
@@ -282,6 +279,9 @@ struct Slot {
 #pragma unroll
             for (int j = 0; j < KD; j++) o[i][j] = (f32x4){0, 0, 0, 0};
         }
+    }
+
+    __device__ __forceinline__ void queries(const RowArgs& a, const TreeAttn& t, const Item& it, int lane) {
         if (!on) return;
         const int r = lane & 15, g = lane >> 4, Q = nr * G;
 #pragma unroll
@@ -530,35 +530,56 @@ __global__ __launch_bounds__(512) void k_tree_attn(RowArgs a, KvLayer kv, TreeAt
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // what depends on it stays scalar
     const int slot = wave % a.rw, share = wave / a.rw;
     Slot<HD, FMT, QT> s;
-    s.start(a, t, it, kv.nkv, blockIdx.x % kv.nkv, slot, lane);
+    s.place(t, it, kv.nkv, blockIdx.x % kv.nkv, slot);
     const int pairs = (s.last - it.page0 + 1) / 2, mine = s.on ? (pairs - share + a.pw - 1) / a.pw : 0;
-    for (int c0 = 0; c0 < mine; c0 += 32) {
-        // the chunk's block ids, two pages a pair; past the last page the last again
+    int ids = 0;  // a chunk's block ids, two pages a pair; past the last page the last again
+    auto chunk = [&](int c0) {
         const int pg = it.page0 + 2 * (share + a.pw * (c0 + lane / 2)) + (lane & 1);
-        const int ids = a.btab[it.btab + min(pg, s.last - 1)];
+        ids = a.btab[it.btab + max(min(pg, s.last - 1), 0)];
+    };
+    auto block = [&](int c, int x) { return (size_t)(uint32_t)__builtin_amdgcn_readlane(ids, 2 * c + x); };
+    // AHEAD: keys and values are asked for as soon as the registers of the pair before are free, the keys behind
+    // the scores, the values behind the weighted sum. Otherwise the registers do not hold both: the values take
+    // the keys' behind the scores. The first ones go out before the queries are read.
+    constexpr bool AHEAD = HD < 128 || (QT == 1 && FMT != KV_F32);
+    KeyPage<HD, FMT> kp[2];
+    ValuePage<HD, FMT> vp[2];
+    auto first = [&](int c0) {
+        if (c0 >= mine) return;
+        chunk(c0);
+        if constexpr (AHEAD) {
+#pragma unroll
+            for (int x = 0; x < 2; x++) kp[x].load(kv, block(0, x), s.h, lane);
+#pragma unroll
+            for (int x = 0; x < 2; x++) vp[x].load(kv, block(0, x), s.h, lane);
+        }
+    };
+    first(0);
+    s.queries(a, t, it, lane);
+    for (int c0 = 0; c0 < mine; c0 += 32) {
         const int np = min(32, mine - c0);
-        auto block = [&](int c, int x) { return (size_t)(uint32_t)__builtin_amdgcn_readlane(ids, 2 * c + x); };
-        // keys and values are asked for as soon as the registers of the pair before are free: the keys behind
-        // the scores, the values behind the weighted sum
-        KeyPage<HD, FMT> kp[2];
-        ValuePage<HD, FMT> vp[2];
-#pragma unroll
-        for (int x = 0; x < 2; x++) kp[x].load(kv, block(0, x), s.h, lane);
-#pragma unroll
-        for (int x = 0; x < 2; x++) vp[x].load(kv, block(0, x), s.h, lane);
+        if (c0) first(c0);
         for (int c = 0; c < np; c++) {
             const int next = min(c + 1, np - 1);
             float raw[QT][8], vsc[8], vf[8];
+            if constexpr (!AHEAD)
+#pragma unroll
+                for (int x = 0; x < 2; x++) kp[x].load(kv, block(c, x), s.h, lane);
             s.scores(kp, raw, lane);
 #pragma unroll
-            for (int x = 0; x < 2; x++) kp[x].load(kv, block(next, x), s.h, lane);
+            for (int x = 0; x < 2; x++)
+                if constexpr (AHEAD)
+                    kp[x].load(kv, block(next, x), s.h, lane);
+                else
+                    vp[x].load(kv, block(c, x), s.h, lane);
 #pragma unroll
             for (int x = 0; x < 2; x++) value_scales<HD, FMT>(vp[x], &vsc[4 * x], &vf[4 * x]);
             f16x8 hi[QT], lo[QT];
             s.weights(a, it, it.page0 + 2 * (share + a.pw * (c0 + c)), raw, vsc, hi, lo, lane);
             s.gather(hi, lo, vp, vf);
+            if constexpr (AHEAD)
 #pragma unroll
-            for (int x = 0; x < 2; x++) vp[x].load(kv, block(next, x), s.h, lane);
+                for (int x = 0; x < 2; x++) vp[x].load(kv, block(next, x), s.h, lane);
         }
     }
     s.join(sh, slot, share, a.rw, a.pw, lane);
@@ -591,7 +612,7 @@ __global__ __launch_bounds__(512) void k_tree_attn_lds(RowArgs a, KvLayer kv, Tr
     const int pages = it.page1 - it.page0, stages = (pages + PPS - 1) / PPS;
     for (int i = threadIdx.x; i < pages; i += 64 * W) ids[i] = a.btab[it.btab + it.page0 + i];
     Slot<HD, FMT, QT> s;
-    s.start(a, t, it, kv.nkv, blockIdx.x % kv.nkv, slot, lane);
+    s.place(t, it, kv.nkv, blockIdx.x % kv.nkv, slot);
     __syncthreads();
     // the wave's copies of a stage: codes copy i of page `page`, from byte `off` of its record to byte `to` of the
     // stage; more copies than there are repeat the last
@@ -655,6 +676,7 @@ __global__ __launch_bounds__(512) void k_tree_attn_lds(RowArgs a, KvLayer kv, Tr
         }
     };
     for (int i = 0; i < NST - 1; i++) copy(i);
+    s.queries(a, t, it, lane);
     // This wave's copies of all stages but the last `left` have landed, then everyone's.
 #define LANDED(left)                                                                               \
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"((left) * (COPIES + SCOPIES)) : "memory");              \
