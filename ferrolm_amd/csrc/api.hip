@@ -2514,7 +2514,7 @@ static int rows_plan(fg_rows* r, const fg_tree_seq* seqs, int32_t n_seqs) {
     if ((rc = ensure(&r->hmeta, &r->hmeta_cap, P.words * 4, r->ctx->stream, true)) ||
         (rc = ensure(&r->dmeta, &r->dmeta_cap, P.words * 4, r->ctx->stream, false)))
         return rc;
-    if (P.parts && (rc = ensure(&r->part, &r->part_cap,
+    if (P.parts > 1 && (rc = ensure(&r->part, &r->part_cap,
                                 (size_t)P.n_wi * r->kv_heads * attn_qmax(r->head_dim) * (r->head_dim + 4) * 4,
                                 r->ctx->stream, false)))
         return rc;

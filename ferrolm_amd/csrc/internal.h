@@ -387,7 +387,8 @@ struct RowArgs {
     const int32_t *cstart = nullptr, *clist = nullptr;  // children of each row, in order
     const int32_t* parent = nullptr;                    // in the row's sequence, -1: none
     int n_seqs = 0, rows = 0, n_items = 0, n_wi = 0, n_quads = 0, longest = 0, most_rows = 0;  // most_rows: of a sequence
-    bool unused = false, parts = false;  // some row is unused; some row has several items
+    int parts = 0;        // most parts of a row's context
+    bool unused = false;  // some row is unused
     int qt = 0, rw = 0, pw = 0;      // 16-query tiles a wave, row slots and position shares a workgroup
 };
 

@@ -31,7 +31,8 @@ struct RowPlan {
     uint32_t top_block = 0;  // the highest block id
     int64_t tokens = 0;  // cached tokens of all sequences, rows among them
     int qt = 1, rw = 1, pw = 1;
-    bool unused = false, parts = false;  // some row is unused; some row has several items
+    int parts = 0;        // most parts of a row's context
+    bool unused = false;  // some row is unused
     bool rooted = true;  // every sequence's rows hang on its first
     std::vector<int32_t> seqs, btab, items, mrec, quads, rpos, cstart, clist, parent;
     std::vector<uint16_t> masks;
@@ -166,7 +167,7 @@ inline void plan_rows(RowPlan& P, const RowSeq* in, int n_seqs, int nh, int nkv,
                 mr[1] = P.n_wi + (i - r0) / rps * np;
                 mr[2] = np;
             }
-            P.parts = P.parts || np > 1;
+            P.parts = std::max(P.parts, np);
             P.n_wi += np * slots;
         }
     auto place = [&](size_t n) {

@@ -712,8 +712,50 @@ __global__ __launch_bounds__(512) void k_tree_attn_lds(RowArgs a, KvLayer kv, Tr
     if (s.on && share == 0) s.finish(a, t, it, kv.nkv, slot, lane);
 }
 
-// The parts of each row's heads: one workgroup per (row, kv head x QH heads),
-// 4 channels a thread, the parts dealt over the rest of the workgroup's threads.
+// The parts of each (row, query head), 4 channels a thread. Up to kFewParts: all of them asked for at once, 256
+// threads for as many pairs as they hold.
+constexpr int kFewParts = 8;
+template <int HD>
+__global__ __launch_bounds__(256) void k_tree_merge_few(RowArgs a, TreeAttn t, int nkv) {
+    constexpr int T = HD / 4, QM = HD >= 64 ? 32 : 64;
+    const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) / T;
+    const int d = threadIdx.x % T, G = t.nh / nkv, row = (int)(at / t.nh), hq = (int)(at % t.nh);
+    if (row >= a.rows) return;
+    const int4 mr = *(const int4*)(a.mrec + (size_t)row * 4);
+    if (mr.z == 1) return;  // written by the attention
+    const size_t stride = (size_t)nkv * QM * (HD + 4);
+    const float* base = t.part + (((size_t)mr.y * nkv + hq / G) * QM + mr.x + hq % G) * (HD + 4);
+    float2 st[kFewParts];
+    float4 v[kFewParts];
+#pragma unroll
+    for (int s = 0; s < kFewParts; s++) {
+        const float* p = base + min(s, mr.z - 1) * stride;
+        st[s] = *(const float2*)p;
+        v[s] = *(const float4*)(p + 4 + 4 * d);
+    }
+    float m = kLowest, l = 0.0f;
+#pragma unroll
+    for (int s = 0; s < kFewParts; s++) {
+        if (s >= mr.z || st[s].x == -INFINITY) st[s] = make_float2(-INFINITY, 0.0f);
+        m = fmaxf(m, st[s].x);
+    }
+    float4 y = make_float4(0, 0, 0, 0);
+#pragma unroll
+    for (int s = 0; s < kFewParts; s++) {
+        const float f = __builtin_amdgcn_exp2f(st[s].x - m);
+        if (s >= mr.z) continue;
+        l += st[s].y * f;
+        y.x += v[s].x * f;
+        y.y += v[s].y * f;
+        y.z += v[s].z * f;
+        y.w += v[s].w * f;
+    }
+    const float f = 1.0f / l;
+    y = l == 0.0f || mr.w ? make_float4(0, 0, 0, 0) : make_float4(y.x * f, y.y * f, y.z * f, y.w * f);
+    *(float4*)(t.out + (size_t)row * t.ldo + (size_t)hq * HD + 4 * d) = y;
+}
+
+// More: one workgroup per pair, the parts dealt over its threads.
 template <int HD>
 __global__ __launch_bounds__(256) void k_tree_merge(RowArgs a, TreeAttn t, int nkv) {
     constexpr int T = HD / 4, NP = 256 / T, QM = HD >= 64 ? 32 : 64;
@@ -797,7 +839,12 @@ static void tree_hd(hipStream_t st, const RowArgs& a, const KvLayer& kv, const T
         tree_qt<HD, KV_INT8>(st, a, kv, t);
     else
         tree_qt<HD, KV_FP8>(st, a, kv, t);
-    if (t.out && a.parts) hipLaunchKernelGGL((k_tree_merge<HD>), dim3(a.rows, t.nh), dim3(256), 0, st, a, t, kv.nkv);
+    if (!t.out || a.parts <= 1) return;
+    const int64_t threads = (int64_t)a.rows * t.nh * (HD / 4);
+    if (a.parts <= kFewParts)
+        hipLaunchKernelGGL((k_tree_merge_few<HD>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st, a, t, kv.nkv);
+    else
+        hipLaunchKernelGGL((k_tree_merge<HD>), dim3(a.rows, t.nh), dim3(256), 0, st, a, t, kv.nkv);
 }
 
 int launch_tree_attn(hipStream_t st, const RowArgs& a, const KvLayer& kv, const TreeAttn& t) {

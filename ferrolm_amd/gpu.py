@@ -727,24 +727,28 @@ class Rows:
             self.close()
 
 
+_dtype_names = {}  # torch's dtypes, whose names take longer to ask for than to look up
+
+
 def _device(ctx: Context, a, what: str, dtype: str, shape: tuple, ld: bool = False):
-    """The address of a device array with torch's attributes (data_ptr, dtype, shape, stride, device), which
+    """The address of a device array with torch's methods (data_ptr, dtype, shape, stride, get_device), which
     must have the type and shape; with ld also the distance of its rows, whose elements must be dense."""
-    if str(a.dtype) not in dtype or tuple(a.shape) != shape:
+    name = _dtype_names.get(a.dtype)
+    if name is None:
+        name = _dtype_names[a.dtype] = str(a.dtype)
+    if name not in dtype or a.shape != shape:
         raise ValueError(f"{what}: expected {dtype} {list(shape)}, got {a.dtype} {list(a.shape)}")
-    if a.device.type != "cuda" or a.device.index != ctx.device:
+    if a.get_device() != ctx.device:  # -1 on the host
         raise ValueError(f"{what}: on {a.device}, the context is on GPU {ctx.device}")
     if not ld:
         if not a.is_contiguous():
             raise ValueError(f"{what}: must be contiguous")
         return a.data_ptr()
+    rows, heads, width = shape
     st = a.stride()
-    dense = 1
-    for n, d in zip(shape[:0:-1], st[:0:-1]):
-        if n > 1 and d != dense:
-            raise ValueError(f"{what}: each row must be dense")
-        dense *= n
-    return a.data_ptr(), (st[0] if shape[0] > 1 else dense)
+    if (width > 1 and st[2] != 1) or (heads > 1 and st[1] != width):
+        raise ValueError(f"{what}: each row must be dense")
+    return a.data_ptr(), (st[0] if rows > 1 else heads * width)
 
 
 def _need_cache(rows: Rows, kv: KvCache) -> None:
