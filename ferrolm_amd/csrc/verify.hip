@@ -26,13 +26,33 @@ constexpr int kVerifyThreads = 1024, kVerifyWaves = kVerifyThreads / 64;
 // about that.
 constexpr double kSpent = 0x1p-20;
 
+// Sums over aligned groups of 16 or 64 lanes without the LDS crossbar (devutil.h's lane swaps, a half at a time).
+template <int CTRL>
+__device__ __forceinline__ double dpp_d(double v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, 0xf, 0xf, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), CTRL, 0xf, 0xf, false);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ double row_sum(double x) {
+    x += dpp_d<0xB1>(x);   // quad_perm [1,0,3,2]
+    x += dpp_d<0x4E>(x);   // quad_perm [2,3,0,1]
+    x += dpp_d<0x141>(x);  // row_half_mirror
+    return x + dpp_d<0x140>(x);  // row_mirror
+}
 __device__ __forceinline__ double wave_sum(double x) {
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) x += __shfl_xor(x, m);
-    return x;
+    x = row_sum(x);
+    uint64_t b = __builtin_bit_cast(uint64_t, x);
+    const auto l = __builtin_amdgcn_permlane16_swap((uint32_t)b, (uint32_t)b, false, false);
+    const auto h = __builtin_amdgcn_permlane16_swap((uint32_t)(b >> 32), (uint32_t)(b >> 32), false, false);
+    x = __builtin_bit_cast(double, (uint64_t)h[0] << 32 | l[0]) + __builtin_bit_cast(double, (uint64_t)h[1] << 32 | l[1]);
+    b = __builtin_bit_cast(uint64_t, x);
+    const auto m = __builtin_amdgcn_permlane32_swap((uint32_t)b, (uint32_t)b, false, false);
+    const auto n = __builtin_amdgcn_permlane32_swap((uint32_t)(b >> 32), (uint32_t)(b >> 32), false, false);
+    return __builtin_bit_cast(double, (uint64_t)n[0] << 32 | m[0]) + __builtin_bit_cast(double, (uint64_t)n[1] << 32 | m[1]);
 }
 // x > 0, or 0: a NaN counts as 0
-__device__ __forceinline__ double mass_of(float x) { return x > 0.0f ? (double)x : 0.0; }
+__device__ __forceinline__ double mass_of(float x) { return (double)fmaxf(x, 0.0f); }
 
 // What is left of a node's distribution.
 struct Left {
@@ -79,14 +99,14 @@ __device__ __forceinline__ double share_sum(const Left& f, const Gone& gone, int
         for (int k = 0; k < UN; k++) {
             const int t = min(b + (k * 64 + lane) * E, t1 - E);
             if constexpr (V4) {
-                const f32x4 pv = __builtin_nontemporal_load((const f32x4*)(f.p + t));
+                const f32x4 pv = *(const f32x4*)(f.p + t);
                 f32x4 qv = (f32x4){0, 0, 0, 0};
-                if (Q) qv = __builtin_nontemporal_load((const f32x4*)(f.q + t));
+                if (Q) qv = *(const f32x4*)(f.q + t);
 #pragma unroll
                 for (int e = 0; e < 4; e++) x[k][e] = pv[e], y[k][e] = qv[e];
             } else {
-                x[k][0] = __builtin_nontemporal_load(f.p + t);
-                y[k][0] = Q ? __builtin_nontemporal_load(f.q + t) : 0.0f;
+                x[k][0] = f.p[t];
+                y[k][0] = Q ? f.q[t] : 0.0f;
             }
         }
         if constexpr (!Q)
@@ -96,12 +116,16 @@ __device__ __forceinline__ double share_sum(const Left& f, const Gone& gone, int
 #pragma unroll
                     for (int e = 0; e < E; e++) x[k][e] = b + (k * 64 + lane) * E + e == g ? 0.0f : x[k][e];
             });
+        if (b + UN * E * 64 > t1) {
 #pragma unroll
-        for (int k = 0; k < UN; k++) {
-            const float in = b + (k * 64 + lane) * E < t1 ? 1.0f : 0.0f;  // a NaN stays one, and counts as 0
+            for (int k = 0; k < UN; k++)
 #pragma unroll
-            for (int e = 0; e < E; e++) s[V4 ? e : k & 3] += f.of<Q>(x[k][e] * in, y[k][e]);
+                for (int e = 0; e < E; e++) x[k][e] = b + (k * 64 + lane) * E < t1 ? x[k][e] : 0.0f;
         }
+#pragma unroll
+        for (int k = 0; k < UN; k++)
+#pragma unroll
+            for (int e = 0; e < E; e++) s[V4 ? e : k & 3] += f.of<Q>(x[k][e], y[k][e]);
     }
     return (s[0] + s[1]) + (s[2] + s[3]);
 }
@@ -115,9 +139,8 @@ __device__ double shares(const Left& f, const Gone& gone, int first, int last, d
     __syncthreads();  // the sums of the call before have been read
     if (lane == 0) sums[wave] = x;
     __syncthreads();
-    double total = 0.0;
-    for (int w = 0; w < kVerifyWaves; w++) total += sums[w];
-    return total;
+    static_assert(kVerifyWaves == 16, "a row of lanes");
+    return row_sum(sums[lane & 15]);
 }
 // The share in which the cumulative sum passes `target`, which becomes relative to the share's start; where
 // rounding leaves none, the last share with any mass.
@@ -249,6 +272,7 @@ __global__ __launch_bounds__(kVerifyThreads) void k_tree_verify(RowArgs a, Verif
         for (int i = tid; i < gone.n; i += kVerifyThreads) g[i] = tr.tok[tr.clist[tr.cstart[node] + i]];
         __syncthreads();
     }
+    if (left.a == 0.0) left.q = nullptr;  // nothing was taken from p: its row alone
     if (!known) total = shares<V4>(left, gone, 0, V, sums);
     if (!(total > 0.0)) {  // nothing is left: the target's own distribution
         left.a = 0.0;
@@ -256,35 +280,46 @@ __global__ __launch_bounds__(kVerifyThreads) void k_tree_verify(RowArgs a, Verif
         gone.n = 0;
         total = shares<V4>(left, gone, 0, V, sums);
     }
+    // the share that the target falls in, then its tokens in order, eight a thread
     double target = (double)tr.u[0] * total;
-    int first = 0, last = V;
-    for (int round = 0; round < 2; round++) {
-        if (round) (void)shares<V4>(left, gone, first, last, sums);
-        const int w = pick(sums, target), len = share_len<V4>(last - first);
-        first += w * len;
-        last = max(first, min(last, first + len));
+    const int len = share_len<V4>(V), first = pick(sums, target) * len, last = min(V, first + len), wave = tid >> 6;
+    __shared__ int found, positive;
+    if (tid == 0) {
+        found = INT32_MAX;
+        positive = 0;
     }
-    if (tid >= 64) return;
-    // one wave, in token order: a lane's consecutive tokens, eight at a time
-    int found = -1, positive = 0;
-    double c = 0.0;
-    for (int t0 = first; t0 < last && found < 0; t0 += 512) {
-        double w[8], mine = 0.0;
+    double before = 0.0;
+    for (int c0 = first; c0 < last; c0 += 8 * kVerifyThreads) {
         float px[8], qx[8];
+        const int t0 = c0 + 8 * tid;
+        if constexpr (V4) {
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const int t = min(t0 + 8 * lane + e, last - 1);
-            px[e] = left.p[t];
-            qx[e] = left.q ? left.q[t] : 0.0f;
+            for (int k = 0; k < 2; k++) {
+                const int t = min(t0 + 4 * k, last - 4);
+                const f32x4 x = *(const f32x4*)(left.p + t);
+                f32x4 y = (f32x4){0, 0, 0, 0};
+                if (left.q) y = *(const f32x4*)(left.q + t);
+#pragma unroll
+                for (int e = 0; e < 4; e++) px[4 * k + e] = x[e], qx[4 * k + e] = y[e];
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const int t = min(t0 + e, last - 1);
+                px[e] = left.p[t];
+                qx[e] = left.q ? left.q[t] : 0.0f;
+            }
         }
-        gone.each(t0, t0 + 512, [&](int g) {
+        const int w0 = c0 + 512 * wave;
+        gone.each(w0, w0 + 512, [&](int g) {
 #pragma unroll
-            for (int e = 0; e < 8; e++) px[e] = t0 + 8 * lane + e == g ? 0.0f : px[e];
+            for (int e = 0; e < 8; e++) px[e] = t0 + e == g ? 0.0f : px[e];
         });
+        double w[8], mine = 0.0;
 #pragma unroll
         for (int e = 0; e < 8; e++) {
             const double x = left.q ? left.of<true>(px[e], qx[e]) : left.of<false>(px[e], 0.0f);
-            w[e] = t0 + 8 * lane + e < last ? x : 0.0;
+            w[e] = t0 + e < last ? x : 0.0;
             mine += w[e];
         }
         double x = mine;
@@ -293,26 +328,33 @@ __global__ __launch_bounds__(kVerifyThreads) void k_tree_verify(RowArgs a, Verif
             const double y = __shfl_up(x, m);
             if (lane >= m) x += y;
         }
-        double run = c + (x - mine);
-        int hit = -1, top = -1;
+        __syncthreads();  // the sums before have been read
+        if (lane == 63) sums[wave] = x;
+        __syncthreads();
+        double run = before;
+        for (int i = 0; i < wave; i++) run += sums[i];
+        run += x - mine;
+        int hit = INT32_MAX, top = -1;
 #pragma unroll
         for (int e = 0; e < 8; e++) {
             run += w[e];
             if (w[e] > 0.0) {
-                top = t0 + 8 * lane + e;
-                if (hit < 0 && run > target) hit = top;
+                top = t0 + e;
+                if (hit == INT32_MAX && run > target) hit = top;
             }
         }
-        const uint64_t hits = __ballot(hit >= 0), tops = __ballot(top >= 0);
-        if (tops) positive = __shfl(top, 63 - __builtin_clzll(tops));
-        if (hits) found = __shfl(hit, __builtin_ctzll(hits));
-        c += __shfl(x, 63);
+        const uint64_t hits = __ballot(hit != INT32_MAX), tops = __ballot(top >= 0);
+        if (hits && lane == __builtin_ctzll(hits)) atomicMin(&found, hit);
+        if (tops && lane == 63 - __builtin_clzll(tops)) atomicMax(&positive, top);
+        for (int i = 0; i < kVerifyWaves; i++) before += sums[i];
+        __syncthreads();
+        if (found != INT32_MAX) break;
     }
-    if (lane == 0) {
-        out[count - 1] = (uint32_t)(found >= 0 ? found : positive);
+    if (tid == 0) {
+        out[count - 1] = (uint32_t)(found != INT32_MAX ? found : positive);
         v.out_count[s] = count;
     }
-    for (int i = count + lane; i < v.ld; i += 64) {
+    for (int i = count + tid; i < v.ld; i += kVerifyThreads) {
         out[i] = 0;
         path[i] = -1;
     }
