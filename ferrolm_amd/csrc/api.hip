@@ -281,7 +281,7 @@ struct fg_model {
 struct fg_kv {
     uint64_t serial = g_serial++;
     int layers = 0, kv_heads = 0, head_dim = 0, block_size = 0, blocks = 0;
-    int format = KV_F32;
+    int format = KV_F32, device = 0;
     float* k = nullptr;  // [layer][blocks*bs*nkv*hd]
     float* v = nullptr;
     uint8_t* data = nullptr;  // 8-bit formats: [layer][block][kv head][record]
@@ -1562,6 +1562,7 @@ int fg_kv_create_format(fg_ctx* ctx, int32_t layers, int32_t kv_heads, int32_t h
     kv->block_size = block_size;
     kv->blocks = blocks;
     kv->format = format;
+    kv->device = ctx->device;
     const size_t bytes = kv->layer_bytes() * layers;
     const bool ok = format == FG_KV_F32
                         ? hipMalloc((void**)&kv->k, bytes) == hipSuccess && hipMalloc((void**)&kv->v, bytes) == hipSuccess
@@ -2486,9 +2487,13 @@ static int check_parents(const int32_t* parents, int32_t n, bool unused) {
 static int rows_plan(fg_rows* r, const fg_tree_seq* seqs, int32_t n_seqs) {
     if (n_seqs < 0 || (n_seqs > 0 && !seqs)) return fail(FG_E_ARG, "null sequences");
     if (n_seqs > 65535) return fail(FG_E_SHAPE, "at most 65535 sequences");
+    // the copies and allocations below are no part of a graph
+    hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+    HIPCHK(hipStreamIsCapturing(r->ctx->stream, &cap));
+    if (cap != hipStreamCaptureStatusNone) return fail(FG_E_ARG, "rows can't be planned while the context's stream is captured");
     const bool cached = r->kv_blocks > 0;
     std::vector<RowSeq> in(n_seqs);
-    int64_t rows = 0, tokens = 0;
+    int64_t rows = 0, tokens = 0, masks = 0;
     for (int s = 0; s < n_seqs; s++) {
         const fg_tree_seq& q = seqs[s];
         if (q.n < 0 || q.pos < 0) return fail(FG_E_ARG, "negative row count or position");
@@ -2503,9 +2508,11 @@ static int rows_plan(fg_rows* r, const fg_tree_seq* seqs, int32_t n_seqs) {
         }
         rows += q.n;
         tokens += last;
+        masks += q.parents && q.n <= kTreeRows ? (int64_t)q.n * (q.n / 16 + 2) : 0;  // at most
         in[s] = RowSeq{q.n, q.pos, q.blocks, q.n_blocks, q.parents};
     }
-    if (rows > (1 << 24) || tokens > INT32_MAX) return fail(FG_E_SHAPE, "too many rows or tokens");
+    if (rows > (1 << 24) || tokens > INT32_MAX || masks > INT32_MAX) return fail(FG_E_SHAPE, "too many rows or tokens");
+    r->ready = false;  // a refusal above leaves the plan before
     plan_rows(r->plan, in.data(), n_seqs, r->heads, r->kv_heads, r->head_dim, cached);
     const RowPlan& P = r->plan;
     // the staging may still be on its way up for the plan before
@@ -2560,10 +2567,6 @@ int fg_rows_create(fg_ctx* ctx, const fg_kv* kv, int32_t heads, const fg_tree_se
 int fg_rows_set(fg_rows* r, const fg_tree_seq* seqs, int32_t n_seqs) {
     if (!r) return fail(FG_E_ARG, "null rows");
     const DeviceScope on(r->ctx->device);
-    hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
-    HIPCHK(hipStreamIsCapturing(r->ctx->stream, &cap));
-    if (cap != hipStreamCaptureStatusNone) return fail(FG_E_ARG, "rows can't be planned while the context's stream is captured");
-    r->ready = false;
     return guarded([&] { return rows_plan(r, seqs, n_seqs); });
 }
 
@@ -2590,6 +2593,7 @@ int fg_rows_count(const fg_rows* r, int32_t* rows, int64_t* tokens, int32_t* dee
 static int check_rows(const fg_ctx* ctx, const fg_rows* r, const fg_kv* kv, int32_t layer) {
     if (!ctx || !r || !kv) return fail(FG_E_ARG, "null argument");
     if (r->ctx != ctx || !r->ready) return fail(FG_E_ARG, "the rows are another context's, or without a plan");
+    if (kv->device != ctx->device) return fail(FG_E_ARG, "the cache is another device's");
     if (layer < 0 || layer >= kv->layers) return fail(FG_E_ARG, "no such layer");
     if (!r->kv_blocks || r->kv_heads != kv->kv_heads || r->head_dim != kv->head_dim)
         return fail(FG_E_SHAPE, "the rows were planned for another cache shape");

@@ -374,7 +374,8 @@ int fg_rows_create(fg_ctx* ctx, const fg_kv* kv, int32_t heads,
                    const fg_tree_seq* seqs, int32_t n_seqs, fg_rows** out);
 /* Plans other rows in the same handle (the next step's); calls queued before
  * keep theirs. Graphs that captured calls with the handle are void after it.
- * Refused (FG_E_ARG) while the context's stream is captured. */
+ * A refused plan leaves the one before. Refused (FG_E_ARG), as fg_rows_create
+ * is, while the context's stream is captured. */
 int fg_rows_set(fg_rows* rows, const fg_tree_seq* seqs, int32_t n_seqs);
 void fg_rows_destroy(fg_rows* rows);
 /* Rows, cached tokens with the rows among them, and rows on the longest
