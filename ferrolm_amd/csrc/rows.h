@@ -114,8 +114,8 @@ inline void plan_rows(RowPlan& P, const RowSeq* in, int n_seqs, int nh, int nkv,
         if (q.n) {
             most_q = std::max(most_q, std::min(q.n, rps) * G);
             most_slots = std::max(most_slots, (q.n + rps - 1) / rps);
-            P.longest = std::max(P.longest, L);
         }
+        P.longest = std::max(P.longest, L);
         P.rows += q.n;
         P.tokens += L;
     }
