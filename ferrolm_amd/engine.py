@@ -155,6 +155,7 @@ class EngineConfig:
     admission: str = "continuous"  # or "static"
     reserve_tokens: int | None = None  # slots reserved per sequence at admission
     spec_k: int = 4
+    kv_format: str = "f32"  # of both caches (gpu.KV_FORMATS); the reference has f32 ones
 
 
 @dataclass
@@ -242,14 +243,14 @@ class Engine:
         if cfg.block_size != 16:
             raise ValueError("the device caches use 16-token blocks")
         c = model.cfg
-        self.kv = gpu.KvCache(ctx, c, cfg.kv_blocks)
+        self.kv = gpu.KvCache(ctx, c, cfg.kv_blocks, format=cfg.kv_format)
         self.blocks = BlockManager(cfg.kv_blocks, cfg.block_size, cfg.prefix_cache)
         self.tables = TableCache()  # uint32 copies of the running sequences' block tables
         if draft is not None:
             if draft.cfg.vocab != c.vocab:
                 raise ValueError("draft and target must share a vocabulary")
             n = cfg.kv_blocks + cfg.max_seqs  # as many slots as the target, plus room for proposals
-            self.dkv = gpu.KvCache(ctx, draft.cfg, n)
+            self.dkv = gpu.KvCache(ctx, draft.cfg, n, format=cfg.kv_format)
             self.dblocks = BlockManager(n, cfg.block_size, False)
         self.max_len = min(c.max_position, cfg.kv_blocks * cfg.block_size)
         self.waiting: deque = deque()

@@ -242,3 +242,107 @@ def test_a_tree_run_ends_at_the_context_limit(ctx):
     m = gpu.Model(ctx, hm)
     r = generate_tree(ctx, m, m.truncated(1), prompt(20, hm.cfg.vocab), 500, (2, 2), kv_blocks=4)
     assert len(r) == 4 * 16 - 20
+
+
+def shaped(kind, hidden, heads, kv_heads, hd, inter, seed, bias=False):
+    from ferrolm_amd import synth
+    from ferrolm_amd.weights import Config
+    c = Config(vocab=608, hidden=hidden, intermediate=inter, layers=2, heads=heads, kv_heads=kv_heads, head_dim=hd,
+               rms_eps=1e-5, rope_theta=1e4, max_position=1024, tie_embeddings=True, qkv_bias=bias, eos=(0,))
+    return synth.quantize_model(synth.random_model(c, seed), kind)
+
+
+@pytest.mark.parametrize("fmt", gpu.KV_FORMATS)
+@pytest.mark.parametrize("kind,shape", [(0, (576, 9, 3, 64, 1536)), (2, (1024, 16, 16, 64, 2048)),
+                                        (1, (1024, 16, 2, 128, 1024)), (0, (256, 8, 1, 32, 512))])
+def test_wide_models_over_every_cache(ctx, fmt, kind, shape):
+    """Head dims and weight kinds of the served models, through the fused small steps, the GEMVs and the GEMMs:
+    prompt, decode rows of several sequences, trees."""
+    hm = shaped(kind, *shape, seed=shape[0])
+    c, m = hm.cfg, gpu.Model(ctx, hm)
+    kv = gpu.KvCache(ctx, c, 64, format=fmt)
+    tables = [[3 * i + s for i in range(12)] for s in range(3)]
+    toks = [prompt(150, c.vocab, 40 + s) for s in range(3)]
+    at = [0, 0, 0]
+
+    def check(rows, call):
+        """rows: per sequence the parents of its rows"""
+        o = call([toks[s][at[s]:at[s] + len(rows[s])] for s in range(3)])
+        i = 0
+        for s in range(3):
+            n, p = at[s], rows[s]
+            vis, depth = np.zeros((len(p), n + len(p)), bool), []
+            for j, x in enumerate(p):
+                depth.append(0 if x < 0 else depth[x] + 1)
+                vis[j] = vis[x] if x >= 0 else np.arange(n + len(p)) < n
+                vis[j, n + j] = True
+            want, own = forward64(hm, toks[s][n:n + len(p)], n + np.array(depth), vis, held(kv, c, tables[s], n + len(p)))
+            check_cached(own, [(k[n:], v[n:]) for k, v in held(kv, c, tables[s], n + len(p))], fmt)
+            got = o.logits[i:i + len(p)]
+            assert np.abs(got - want).max() <= LOGIT_TOL * np.abs(want).max()
+            i += len(p)
+    for n in ((70, 33, 9), (1, 1, 1), (2, 1, 1), (3, 5, 12)):
+        check([list(range(-1, k - 1)) for k in n],
+              lambda t: gpu.forward(ctx, m, kv, [(t[s], at[s], tables[s], gpu.LOGITS_ALL) for s in range(3)]))
+        at = [a + k for a, k in zip(at, n)]
+    trees = [[-1, 0, 0, 1], [-1, -1, 0, 1, 1, 2, 2, 6], [-1]]
+    check(trees, lambda t: gpu.forward_tree(ctx, m, kv, [gpu.TreeSeq(at[s], tables[s], trees[s], t[s]) for s in range(3)]))
+
+
+@pytest.mark.parametrize("fmt", ["int8", "fp8"])
+def test_speculative_steps_on_8_bit_caches_with_and_without_graphs(ctx, fmt, monkeypatch):
+    """The same launches captured and direct: the same tokens, over enough steps that contexts pass block and
+    plan boundaries."""
+    hm = shaped(0, 576, 9, 3, 64, 1536, seed=5)
+    outs = []
+    for no_graph in ("0", "1"):
+        monkeypatch.setenv("FERRO_NO_GRAPH", no_graph)
+        x = gpu.Context(0)
+        m = gpu.Model(x, hm)
+        d = m.truncated(1)
+        p = prompt(30, hm.cfg.vocab)
+        outs.append(generate(x, m, d, p, 120, 3, kv_blocks=32, tkv=gpu.KvCache(x, hm.cfg, 32, format=fmt),
+                             dkv=gpu.KvCache(x, d.cfg, 96, format=fmt)))
+    assert np.array_equal(outs[0], outs[1])
+
+
+@pytest.mark.parametrize("fmt", ["int8", "fp8"])
+def test_capture_on_an_8_bit_cache(ctx, fmt):
+    """The first layer's attention rows of a calibration capture: over what the cache holds."""
+    hm = load_model(GOLDEN / "llama-gqa")
+    c, m, p = hm.cfg, gpu.Model(ctx, hm), prompt(37, hm.cfg.vocab)
+    kv = gpu.KvCache(ctx, c, 8, format=fmt)
+    x, got = gpu.forward_capture(ctx, m, kv, [(p, 0, [4, 1, 2])])[0][:2]
+    (ck, cv), n, l = held(kv, c, [4, 1, 2], 37)[0], 37, hm.layers[0]
+    q = (x.astype(np.float64) @ l.wqkv.to_f32().astype(np.float64).T + (0 if l.bqkv is None else l.bqkv))[:, :c.q_dim]
+    q = rope(c, q.reshape(n, -1, c.head_dim), np.arange(n))
+    want = np.zeros_like(q)
+    for h in range(c.heads):
+        g = h * c.kv_heads // c.heads
+        s = np.where(np.tri(n, dtype=bool), q[:, h] @ ck[:, g].T / np.sqrt(c.head_dim), -np.inf)
+        w = np.exp(s - s.max(1, keepdims=True))
+        want[:, h] = w / w.sum(1, keepdims=True) @ cv[:, g]
+    assert np.abs(got - want.reshape(n, -1)).max() <= LOGIT_TOL * np.abs(want).max()
+
+
+@pytest.mark.parametrize("fmt", ["int8", "fp8"])
+@pytest.mark.parametrize("spec_k", [0, 3])
+def test_the_engine_serves_from_8_bit_caches(ctx, fmt, spec_k):
+    """Requests of a shared prefix, chunked and overlapping, plain and speculative: each one's tokens against the
+    logits of a fresh forward over them, as the generations above."""
+    from ferrolm_amd.engine import Engine, EngineConfig, Params
+    hm = load_model(GOLDEN / "llama-gqa")
+    c, m = hm.cfg, gpu.Model(ctx, hm)
+    e = Engine(ctx, m, m.truncated(1) if spec_k else None,
+               EngineConfig(kv_blocks=64, kv_format=fmt, spec_k=spec_k or 4, max_batch_tokens=40, max_seqs=2))
+    assert e.kv.format == fmt and (not spec_k or e.dkv.format == fmt)
+    first = [int(t) for t in prompt(40, c.vocab, 9)]
+    prompts = [first + [int(t) for t in prompt(3 + 9 * i, c.vocab, i)] for i in range(4)]
+    reqs = [e.submit(p, Params(max_tokens=12, ignore_eos=True)) for p in prompts]
+    e.run_until_idle()
+    for p, r in zip(prompts, reqs):
+        assert len(r.tokens) == 12
+        whole = p + [int(t) for t in r.tokens]
+        o = gpu.forward(ctx, m, gpu.KvCache(ctx, c, 8, format=fmt), [(whole[:-1], 0, list(range(8)), gpu.LOGITS_ALL)])
+        lg = o.logits[len(p) - 1:]
+        assert (lg.max(1) - lg[np.arange(12), r.tokens] <= (STEP[fmt] / 32 + 2 * LOGIT_TOL) * np.abs(lg).max(1)).all()
