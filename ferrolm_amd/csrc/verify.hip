@@ -205,16 +205,22 @@ __global__ __launch_bounds__(kVerifyThreads) void k_tree_verify(RowArgs a, Verif
         tr.u[i] = v.u[row0 + i];
         tr.p[i] = in ? v.p[at] : 0.0f;
         tr.q[i] = in ? (v.kind == DRAFT_FIXED ? 1.0f : v.q[at]) : 0.0f;
-        tr.seen[i] = 0;
+        tr.seen[i] = parent;
     }
     __syncthreads();
     for (int i = tid; i < tr.cstart[n]; i += kVerifyThreads) tr.clist[i] = a.clist[c0 + i] - row0;
     __syncthreads();
     if (v.kind != DRAFT_EACH) {
-        for (int i = tid; i < n; i += kVerifyThreads)
-            for (int j = tr.cstart[i] + 1; j < tr.cstart[i + 1]; j++)
-                for (int k = tr.cstart[i]; k < j; k++)
-                    if (tr.tok[tr.clist[k]] == tr.tok[tr.clist[j]]) tr.seen[tr.clist[j]] = 1;
+        for (int i = tid; i < n; i += kVerifyThreads) {
+            const int parent = tr.seen[i];
+            if (parent < 0) {
+                tr.seen[i] = 0;
+                continue;
+            }
+            int seen = 0;
+            for (int k = tr.cstart[parent], c; (c = tr.clist[k]) != i; k++) seen |= tr.tok[c] == tr.tok[i];
+            tr.seen[i] = seen;
+        }
         __syncthreads();
     }
     int node = 0, count = 1;
@@ -231,11 +237,11 @@ __global__ __launch_bounds__(kVerifyThreads) void k_tree_verify(RowArgs a, Verif
         int passed = -1;
         for (int j = tr.cstart[node]; j < tr.cstart[node + 1] && passed < 0; j++) {
             const int c = tr.clist[j];
-            const bool seen = tr.seen[c];
+            const bool seen = v.kind != DRAFT_EACH && tr.seen[c];
             const double p = mass_of(tr.p[c]), q = mass_of(tr.q[c]), u = tr.u[c];
             double mass, rate;
             if (v.kind == DRAFT_FIXED) {
-                mass = seen ? 0.0 : p / b;
+                mass = seen || !(b > 0.0) ? 0.0 : p / b;
                 rate = q;
             } else {
                 // without replacement: a token drawn before, or one that q had nothing left for, was not drawn
