@@ -35,7 +35,10 @@ namespace {
 
 constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
 // Below every score; its exponential is 0 against any.
-constexpr float kLowest = -1e30f;
+constexpr float kLowest = -3e38f;
+// Once references pass kFused, scores are rounded before theirs is taken from them: what a fused product keeps of
+// the score would be a whole step of the reference's rounding, and the largest score is to stay its reference.
+constexpr float kFused = 0x1p20f;
 // A weight past kMost, or a probability past kMostP (its value may be zero), raises the reference to where the
 // largest weight is 2^kTop and no probability above 2^kTopP.
 constexpr float kMost = 32768.0f, kMostP = 0x1p60f, kTop = 9.0f, kTopP = 40.0f;
@@ -383,24 +386,27 @@ struct Slot {
 #pragma unroll
         for (int i = 0; i < QT; i++) {
             float p[8], w[8];
-            auto weigh = [&] {  // true in a lane whose weights or probabilities are out of bounds
+            // true in a lane whose weights or probabilities are out of bounds; fused: the score's product is not
+            // rounded before the reference, which was, is taken from it
+            auto weigh = [&](bool fused) {
                 float wm = 0.0f, pm = 0.0f;
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
-                    p[e] = __builtin_amdgcn_exp2f(fmaf(raw[i][e], qf[i], -mq[i]));
+                    p[e] = __builtin_amdgcn_exp2f(fused ? fmaf(raw[i][e], qf[i], -mq[i])
+                                                        : __fadd_rn(__fmul_rn(raw[i][e], qf[i]), -mq[i]));
                     w[e] = p[e] * vsc[e];
                     wm = fmaxf(wm, w[e]);
                     pm = fmaxf(pm, p[e]);
                 }
                 return wm > kMost || pm > kMostP;
             };
-            if (__any(part | weigh())) {
+            if (part || __any(weigh(true))) {
                 if (part) mask(a, it, p0, i, raw[i], lane);
-                if (__any(weigh())) {
+                if (__any(weigh(false))) {
                     float top = -INFINITY;
 #pragma unroll
                     for (int e = 0; e < 8; e++) {
-                        const float sc = raw[i][e] * qf[i];
+                        const float sc = __fmul_rn(raw[i][e], qf[i]);
                         top = fmaxf(top, fmaxf(sc + __builtin_amdgcn_logf(vsc[e]) - kTop, sc - kTopP));
                     }
                     const float mn = fmaxf(mq[i], reduce_rows<true, true>(top)), f = __builtin_amdgcn_exp2f(mq[i] - mn);
@@ -408,7 +414,8 @@ struct Slot {
 #pragma unroll
                     for (int j = 0; j < KD; j++) o[i][j] *= f;
                     mq[i] = mn;
-                    (void)weigh();
+                    if (__any(fabsf(mn) > kFused)) full = INT_MIN;  // every pair this way from now on
+                    (void)weigh(false);
                 }
                 // a value that is not finite has a NaN scale, which must not reach the rows that don't see it
 #pragma unroll

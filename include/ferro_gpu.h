@@ -407,8 +407,10 @@ int fg_kv_commit(fg_ctx* ctx, const fg_rows* rows, fg_kv* kv,
 /* Attention of the rows (Model::attention, src/model.rs:395-432, over
  * trees): out[row][head] = sum over the tokens t that the row sees of
  * softmax_t(q . k_t / sqrt(head_dim)) v_t; q_dev and out_dev
- * [row][head][head_dim]. Unused rows get zeros. Reads the rows' own keys and
- * values from the cache: fg_kv_append comes first. out may be q. */
+ * [row][head][head_dim]. Unused rows get zeros. What is not finite in a
+ * query, or in a token's key or value that it sees, makes its output NaN; what
+ * it does not see is never part of it. Reads the rows' own keys and values
+ * from the cache: fg_kv_append comes first. out may be q. */
 int fg_tree_attention(fg_ctx* ctx, const fg_rows* rows, const fg_kv* kv,
                       int32_t layer, const float* q_dev, int64_t ldq,
                       float* out_dev, int64_t ldo);

@@ -345,3 +345,25 @@ def test_gather_of_sequences_without_rows(ctx):
         ctx.sync()
         assert np.array_equal(k.cpu().numpy(), held(np.concatenate([c.k[s] for s in seqs]), "int8"))
         assert np.array_equal(v.cpu().numpy(), held(np.concatenate([c.v[s] for s in seqs]), "int8"))
+
+
+@pytest.mark.parametrize("fmt", gpu.KV_FORMATS)
+@pytest.mark.parametrize("sign", [-1, 1])
+def test_scores_of_any_size(ctx, fmt, sign):
+    """Scores of +-8e32, all alike: the mean of the values, over waves, parts and pages."""
+    c = Case(ctx, fmt, 2, 64, [(3000, 3), (20, TREES["fan"])], seed=11)
+    for k in c.k:
+        k[:] = 1e16 * sign
+    c.fill()
+    q = np.full((8, 4, 64), 1e16, np.float32)
+    qd, out = cuda(q), torch.empty(8, 4, 64, device="cuda")
+    torch.cuda.synchronize()
+    gpu.tree_attention(ctx, c.rows(4), c.kv, 0, qd, out)
+    ctx.sync()
+    at = 0
+    for n, p, v in zip(c.pos, c.parents, c.v):
+        v = held(v, fmt).astype(np.float64)
+        for i, m in enumerate(sees(n, p)):
+            err = np.abs(out[at + i].cpu().numpy() - v[m].mean(0).repeat(2, 0))
+            assert (err <= bound(0, 0, m.sum(), 2.5) * np.abs(v[m]).mean(0).repeat(2, 0)).all()
+        at += len(p)
