@@ -375,7 +375,7 @@ constexpr int kSeqWords = 8;   // first row, rows, pos, first block in btab, fir
                                // mask words per row, first token of the read-back, tokens cached
 constexpr int kItemWords = 16; // sequence (-1: unused), first row, first and last page, first partial slot, slots
                                // between the item's row slots, row slots, 1: no other item has these rows; the
-                               // first six words of the sequence
+                               // first six words of the sequence; the item that its workgroup takes next, or -1
 constexpr int kPartPages = 1024; // most pages of an item
 struct RowArgs {
     const int32_t *seqs = nullptr, *btab = nullptr, *items = nullptr;

@@ -7,6 +7,7 @@
 
 #include <algorithm>
 #include <cstring>
+#include <functional>
 #include <vector>
 
 namespace fg {
@@ -20,11 +21,18 @@ struct RowSeq {
 
 // Longest tree: its masks hold a bit per row and token of the tree.
 constexpr int kTreeRows = 4096;
-// Workgroups that an attention launch is cut into at most, where it has not more row groups: one a CU. More cost more
-// in the merge than they gain: us of a tree over a long fp8 context in 256, 384, 512 workgroups 149, 196, 170,
+// Workgroups that an attention launch is cut into at most, where it has not many more row groups: one a CU. More cost
+// more in the merge than they gain; cut into even parts of each context, us of a tree over a long fp8 context in 256, 384, 512 workgroups 149, 196, 170,
 // of trees of 16 sequences 70, 82, 79; one token over 32000 fp8 tokens (8 heads, workgroups of four waves) in
 // 256, 512, 1024 21.9, 23.6, 33.4, eight chains of 5 17.5, 19.6, 25.0, one token of 16 sequences 22.7, 20.9, 24.9.
 constexpr int kTreeWorkgroups = 256;
+
+// A workgroup takes pieces of consecutive contexts until its share is full, so that ragged ones end together; a piece
+// costs it this many pages besides its own (queries, the first loads, the join). us of a layer at 0 to 6000 cached
+// tokens, 32 heads over 8 of 128 channels, with one piece of even length a workgroup and with 16, 32, 48 pages:
+// trees of 22 tokens, 16 sequences 73, 67, 63, 68, 8 sequences 37, 40, 37, 37, 40 sequences 137, 103, 100, 108; one
+// token of 16 sequences 26, 28, 24, 25; four prompt chunks of 300 128, 122, 114, 126.
+constexpr int kPieceCost = 32;
 
 struct RowPlan {
     int n_seqs = 0, rows = 0, n_wi = 0, n_items = 0, n_quads = 0, longest = 0, deepest = 0, most_rows = 0;
@@ -123,71 +131,118 @@ inline void plan_rows(RowPlan& P, const RowSeq* in, int n_seqs, int nh, int nkv,
     P.qt = most_q <= 16 ? 1 : qm / 16;
     P.rw = std::min(4, most_slots);
     P.pw = P.rw <= 2 ? 4 : 2;
-    // items: rw slots of rows x a part of the pages that they see, in parts of even length
+    // items: rw slots of rows x a part of the pages that they see
     auto group_pages = [&](const RowSeq& q, int r0) {
         const bool chain = P.seqs[(&q - in) * kSeqWords + 4] < 0;
         const int last = chain ? q.pos + std::min(q.n, r0 + P.rw * rps) : q.pos + q.n;
         return (last + 15) / 16;
     };
-    // the shortest parts, in whole rounds of a workgroup's waves, that make no more workgroups than that
-    const int step = P.rw > 1 ? 4 * P.pw : 2 * P.pw;
-    std::vector<int> groups;  // pages of every row group
-    for (int s = 0; cached && s < n_seqs; s++)
-        for (int r0 = 0; r0 < in[s].n; r0 += P.rw * rps) groups.push_back(group_pages(in[s], r0));
-    auto parts_of = [&](int pages, int len) { return (pages + len - 1) / len; };
-    auto fits = [&](int len) {
-        int64_t n = 0;
-        for (int pages : groups) n += parts_of(pages, len);
-        return n * nkv <= kTreeWorkgroups;
+    struct Group {
+        int seq, row0, pages, np, wi;
     };
-    int lo = 1, hi = kPartPages / step;  // in rounds
-    while (lo < hi) {
+    struct Piece {
+        int group, p0, p1;
+        bool head;  // the first of its workgroup
+    };
+    std::vector<Group> groups;
+    for (int s = 0; cached && s < n_seqs; s++)
+        for (int r0 = 0; r0 < in[s].n; r0 += P.rw * rps) groups.push_back(Group{s, r0, group_pages(in[s], r0), 0, 0});
+    // Pieces of the groups' pages for workgroups of at most `budget` pages, a piece's fixed cost among them, in whole
+    // rounds of a workgroup's waves; how many workgroups that takes.
+    const int step = P.rw > 1 ? 4 * P.pw : 2 * P.pw, most_wgs = std::max(1, kTreeWorkgroups / std::max(1, nkv));
+    // More groups than places: whole ones, a workgroup each, longest first, unless there are few and that leaves
+    // places idle for long (with 4 groups a place, two chunks of 2047 took 306 us in shared pieces, 281 whole).
+    // Workgroups of smaller heads run two on a CU, so theirs stay whole (trees of 16 sequences at 64 channels 50 us,
+    // 68 in pieces).
+    const int64_t n = (int64_t)groups.size();
+    bool whole = n > 2 * most_wgs || (n > most_wgs && P.rw > 1 && hd < 128);
+    std::vector<Piece> pieces;
+    auto cut = [&](int budget, bool keep) {
+        int wgs = 0, left = 0;
+        for (int g = 0; g < (int)groups.size(); g++)
+            for (int p = 0, n = groups[g].pages; p < n;) {
+                const bool head = whole || left < kPieceCost + step;
+                if (head) {
+                    wgs++;
+                    left = budget;
+                }
+                const int take = std::min({n - p, kPartPages, whole ? kPartPages : (left - kPieceCost) / step * step});
+                if (keep) pieces.push_back(Piece{g, p, p + take, head});
+                left -= kPieceCost + (take + step - 1) / step * step;
+                p += take;
+            }
+        return wgs;
+    };
+    int64_t total = 0;
+    for (const Group& g : groups) total += g.pages;
+    int lo = kPieceCost + std::max(step, (int)(total / most_wgs)), hi = lo;
+    while (!whole && cut(hi, false) > most_wgs) hi *= 2;
+    while (!whole && lo < hi) {
         const int mid = (lo + hi) / 2;
-        if (fits(mid * step))
+        if (cut(mid, false) <= most_wgs)
             hi = mid;
         else
             lo = mid + 1;
     }
-    const int len = lo * step;
-    for (int s = 0; cached && s < n_seqs; s++)
-        for (int r0 = 0; r0 < in[s].n; r0 += P.rw * rps) {
-            const RowSeq& q = in[s];
-            const int pages = group_pages(q, r0), parts = parts_of(pages, len);
-            const int per = ((pages + parts - 1) / parts + step - 1) / step * step;
-            const int np = parts_of(pages, per), slots = std::min(P.rw, (q.n - r0 + rps - 1) / rps);
-            for (int p = 0; p < np; p++) {
-                const int32_t* sr = &P.seqs[(size_t)s * kSeqWords];
-                const int32_t rec[kItemWords] = {s, r0, p * per, std::min(pages, (p + 1) * per), P.n_wi + p, np, slots,
-                                                 np == 1, sr[0], sr[1], sr[2], sr[3], sr[4], sr[5], 0, 0};
-                P.items.insert(P.items.end(), rec, rec + kItemWords);
-                P.n_items++;
-            }
-            for (int i = r0; i < std::min(q.n, r0 + P.rw * rps); i++) {
-                int32_t* mr = &P.mrec[(size_t)(P.seqs[s * kSeqWords] + i) * 4];
-                mr[1] = P.n_wi + (i - r0) / rps * np;
-                mr[2] = np;
-            }
-            P.parts = std::max(P.parts, np);
-            P.n_wi += np * slots;
+    if (!whole && n > most_wgs) {
+        std::vector<int> len, place(most_wgs, 0);
+        for (const Group& g : groups) len.push_back(g.pages);
+        std::sort(len.begin(), len.end(), std::greater<int>());
+        for (int p : len) *std::min_element(place.begin(), place.end()) += p + kPieceCost;
+        whole = 4 * (int64_t)*std::max_element(place.begin(), place.end()) < 5 * (int64_t)hi;
+    }
+    cut(hi, true);
+    for (const Piece& x : pieces) groups[x.group].np++;
+    for (Group& g : groups) {
+        const RowSeq& q = in[g.seq];
+        const int slots = std::min(P.rw, (q.n - g.row0 + rps - 1) / rps);
+        g.wi = P.n_wi;
+        P.n_wi += g.np * slots;
+        P.parts = std::max(P.parts, g.np);
+        for (int i = g.row0; i < std::min(q.n, g.row0 + P.rw * rps); i++) {
+            int32_t* mr = &P.mrec[(size_t)(P.seqs[g.seq * kSeqWords] + i) * 4];
+            mr[1] = g.wi + (i - g.row0) / rps * g.np;
+            mr[2] = g.np;
+        }
+    }
+    // the launch's items, longest first where they are whole (what is left at the end is short), then those that
+    // follow one in its workgroup; capacities in steps, so that the layout (and a captured step) lasts while contexts
+    // grow
+    std::vector<int> heads;
+    for (int i = 0; i < (int)pieces.size(); i++)
+        if (pieces[i].head) heads.push_back(i);
+    if (whole)
+        std::stable_sort(heads.begin(), heads.end(),
+                         [&](int a, int b) { return pieces[a].p1 - pieces[a].p0 > pieces[b].p1 - pieces[b].p0; });
+    P.n_items = ((int)heads.size() + 15) / 16 * 16;
+    const size_t more = whole ? 0 : (std::max(groups.size(), pieces.size() - heads.size()) + 15) / 16 * 16;
+    P.items.assign((P.n_items + more) * kItemWords, -1);
+    std::vector<int> at(groups.size(), 0);  // parts of a group so far
+    std::vector<int> part(pieces.size());
+    for (int i = 0; i < (int)pieces.size(); i++) part[i] = at[pieces[i].group]++;
+    int follow = P.n_items;
+    auto emit = [&](int i, int slot, int next) {
+        const Piece& x = pieces[i];
+        const Group& g = groups[x.group];
+        const int32_t* sr = &P.seqs[(size_t)g.seq * kSeqWords];
+        const int slots = std::min(P.rw, (in[g.seq].n - g.row0 + rps - 1) / rps);
+        const int32_t rec[kItemWords] = {g.seq, g.row0, x.p0, x.p1, g.wi + part[i], g.np, slots, g.np == 1,
+                                         sr[0], sr[1], sr[2], sr[3], sr[4], sr[5], next, 0};
+        std::copy(rec, rec + kItemWords, P.items.begin() + (size_t)slot * kItemWords);
+    };
+    for (int k = 0; k < (int)heads.size(); k++)
+        for (int i = heads[k], slot = k;; i++) {
+            const bool last = whole || i + 1 == (int)pieces.size() || pieces[i + 1].head;
+            const int next = last ? -1 : follow++;
+            emit(i, slot, next);
+            if (last) break;
+            slot = next;
         }
     auto place = [&](size_t n) {
         const size_t r = P.words;
         P.words += (n + 63) / 64 * 64;
         return r;
     };
-    // longest first: what is left at the end is short
-    std::vector<int> order(P.n_items);
-    for (int i = 0; i < P.n_items; i++) order[i] = i;
-    auto length = [&](int i) { return P.items[(size_t)i * kItemWords + 3] - P.items[(size_t)i * kItemWords + 2]; };
-    std::stable_sort(order.begin(), order.end(), [&](int a, int b) { return length(a) > length(b); });
-    std::vector<int32_t> sorted;
-    for (int i : order)
-        sorted.insert(sorted.end(), P.items.begin() + (size_t)i * kItemWords, P.items.begin() + (size_t)(i + 1) * kItemWords);
-    P.items.swap(sorted);
-    // capacities in steps, so that the layout (and a captured step) lasts while contexts grow; the
-    // added items and quads are unused
-    P.n_items = (P.n_items + 15) / 16 * 16;
-    P.items.resize((size_t)P.n_items * kItemWords, -1);
     P.quads.resize((size_t)P.n_quads * 4, 0);
     P.n_wi = (P.n_wi + 15) / 16 * 16;
     P.btab.resize((P.btab.size() + 255) / 256 * 256, 0);

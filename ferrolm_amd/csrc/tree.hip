@@ -239,15 +239,16 @@ __device__ __forceinline__ void value_scales(const ValuePage<HD, FMT>& p, float*
 // An item's geometry, the same for all of its waves.
 struct Item {
     int seq0, n, pos, btab, mask0, mpages;  // the sequence's record
-    int row0, page0, page1, wi, wi_step, slots, alone;
+    int row0, page0, page1, wi, wi_step, slots, alone, next;  // next: the workgroup's next item, or -1
     bool chain;
     __device__ __forceinline__ bool read(const RowArgs& a, int item) {
-        const int4* p = (const int4*)(a.items + (size_t)item * kItemWords);
-        const int4 i0 = p[0], i1 = p[1], s0 = p[2], s1 = p[3];
-        if (i0.x < 0) return false;  // an unused item of the launch's capacity
-        seq0 = s0.x, n = s0.y, pos = s0.z, btab = s0.w, mask0 = s1.x, mpages = s1.y;
+        // scalar loads, also behind the stores of the item before
+        typedef int words __attribute__((ext_vector_type(16)));
+        const words w = *(const __attribute__((address_space(4))) words*)(uintptr_t)(a.items + (size_t)item * kItemWords);
+        if (w[0] < 0) return false;  // an unused item of the launch's capacity
+        row0 = w[1], page0 = w[2], page1 = w[3], wi = w[4], wi_step = w[5], slots = w[6], alone = w[7];
+        seq0 = w[8], n = w[9], pos = w[10], btab = w[11], mask0 = w[12], mpages = w[13], next = w[14];
         chain = mask0 < 0;
-        row0 = i0.y, page0 = i0.z, page1 = i0.w, wi = i1.x, wi_step = i1.y, slots = i1.z, alone = i1.w;
         return true;
     }
 };
@@ -525,72 +526,75 @@ struct Slot {
 
 }  // namespace
 
-// One workgroup per (kv head, item): rw row slots x pw position shares, a wave
-// each, which takes its pages from memory straight to registers; the shares'
+// One workgroup per (kv head, first item of a list): rw row slots x pw position
+// shares, a wave each, which takes its pages from memory straight to registers; the shares'
 // sums meet in LDS.
 template <int HD, int FMT, int QT>
 __global__ __launch_bounds__(512) void k_tree_attn(RowArgs a, KvLayer kv, TreeAttn t) {
     extern __shared__ float sh[];
     Item it;
-    if (!it.read(a, blockIdx.x / kv.nkv)) return;
-    const int lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // what depends on it stays scalar
-    const int slot = wave % a.rw, share = wave / a.rw;
-    Slot<HD, FMT, QT> s;
-    s.place(t, it, kv.nkv, blockIdx.x % kv.nkv, slot);
-    const int pairs = (s.last - it.page0 + 1) / 2, mine = s.on ? (pairs - share + a.pw - 1) / a.pw : 0;
-    int ids = 0;  // a chunk's block ids, two pages a pair; past the last page the last again
-    auto chunk = [&](int c0) {
-        const int pg = it.page0 + 2 * (share + a.pw * (c0 + lane / 2)) + (lane & 1);
-        ids = a.btab[it.btab + max(min(pg, s.last - 1), 0)];
-    };
-    auto block = [&](int c, int x) { return (size_t)(uint32_t)__builtin_amdgcn_readlane(ids, 2 * c + x); };
-    // AHEAD: keys and values are asked for as soon as the registers of the pair before are free, the keys behind
-    // the scores, the values behind the weighted sum. Otherwise the registers do not hold both: the values take
-    // the keys' behind the scores. The first ones go out before the queries are read.
-    constexpr bool AHEAD = HD < 128 || (QT == 1 && FMT != KV_F32);
-    KeyPage<HD, FMT> kp[2];
-    ValuePage<HD, FMT> vp[2];
-    auto first = [&](int c0) {
-        if (c0 >= mine) return;
-        chunk(c0);
-        if constexpr (AHEAD) {
+    for (int item = blockIdx.x / kv.nkv; item >= 0; item = it.next) {
+        if (!it.read(a, item)) return;
+        int lane = threadIdx.x & 63;
+        asm volatile("" : "+v"(lane));  // an item's addresses are not kept over the others
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // what depends on it stays scalar
+        const int slot = wave % a.rw, share = wave / a.rw;
+        Slot<HD, FMT, QT> s;
+        s.place(t, it, kv.nkv, blockIdx.x % kv.nkv, slot);
+        const int pairs = (s.last - it.page0 + 1) / 2, mine = s.on ? (pairs - share + a.pw - 1) / a.pw : 0;
+        int ids = 0;  // a chunk's block ids, two pages a pair; past the last page the last again
+        auto chunk = [&](int c0) {
+            const int pg = it.page0 + 2 * (share + a.pw * (c0 + lane / 2)) + (lane & 1);
+            ids = a.btab[it.btab + max(min(pg, s.last - 1), 0)];
+        };
+        auto block = [&](int c, int x) { return (size_t)(uint32_t)__builtin_amdgcn_readlane(ids, 2 * c + x); };
+        // AHEAD: keys and values are asked for as soon as the registers of the pair before are free, the keys behind
+        // the scores, the values behind the weighted sum. Otherwise the registers do not hold both: the values take
+        // the keys' behind the scores. The first ones go out before the queries are read.
+        constexpr bool AHEAD = HD < 128 || (QT == 1 && FMT != KV_F32);
+        KeyPage<HD, FMT> kp[2];
+        ValuePage<HD, FMT> vp[2];
+        auto first = [&](int c0) {
+            if (c0 >= mine) return;
+            chunk(c0);
+            if constexpr (AHEAD) {
 #pragma unroll
-            for (int x = 0; x < 2; x++) kp[x].load(kv, block(0, x), s.h, lane);
+                for (int x = 0; x < 2; x++) kp[x].load(kv, block(0, x), s.h, lane);
 #pragma unroll
-            for (int x = 0; x < 2; x++) vp[x].load(kv, block(0, x), s.h, lane);
-        }
-    };
-    first(0);
-    s.queries(a, t, it, lane);
-    for (int c0 = 0; c0 < mine; c0 += 32) {
-        const int np = min(32, mine - c0);
-        if (c0) first(c0);
-        for (int c = 0; c < np; c++) {
-            const int next = min(c + 1, np - 1);
-            float raw[QT][8], vsc[8], vf[8];
-            if constexpr (!AHEAD)
+                for (int x = 0; x < 2; x++) vp[x].load(kv, block(0, x), s.h, lane);
+            }
+        };
+        first(0);
+        s.queries(a, t, it, lane);
+        for (int c0 = 0; c0 < mine; c0 += 32) {
+            const int np = min(32, mine - c0);
+            if (c0) first(c0);
+            for (int c = 0; c < np; c++) {
+                const int next = min(c + 1, np - 1);
+                float raw[QT][8], vsc[8], vf[8];
+                if constexpr (!AHEAD)
 #pragma unroll
-                for (int x = 0; x < 2; x++) kp[x].load(kv, block(c, x), s.h, lane);
-            s.scores(kp, raw, lane);
+                    for (int x = 0; x < 2; x++) kp[x].load(kv, block(c, x), s.h, lane);
+                s.scores(kp, raw, lane);
 #pragma unroll
-            for (int x = 0; x < 2; x++)
+                for (int x = 0; x < 2; x++)
+                    if constexpr (AHEAD)
+                        kp[x].load(kv, block(next, x), s.h, lane);
+                    else
+                        vp[x].load(kv, block(c, x), s.h, lane);
+#pragma unroll
+                for (int x = 0; x < 2; x++) value_scales<HD, FMT>(vp[x], &vsc[4 * x], &vf[4 * x]);
+                f16x8 hi[QT], lo[QT];
+                s.weights(a, it, it.page0 + 2 * (share + a.pw * (c0 + c)), raw, vsc, hi, lo, lane);
+                s.gather(hi, lo, vp, vf);
                 if constexpr (AHEAD)
-                    kp[x].load(kv, block(next, x), s.h, lane);
-                else
-                    vp[x].load(kv, block(c, x), s.h, lane);
 #pragma unroll
-            for (int x = 0; x < 2; x++) value_scales<HD, FMT>(vp[x], &vsc[4 * x], &vf[4 * x]);
-            f16x8 hi[QT], lo[QT];
-            s.weights(a, it, it.page0 + 2 * (share + a.pw * (c0 + c)), raw, vsc, hi, lo, lane);
-            s.gather(hi, lo, vp, vf);
-            if constexpr (AHEAD)
-#pragma unroll
-                for (int x = 0; x < 2; x++) vp[x].load(kv, block(next, x), s.h, lane);
+                    for (int x = 0; x < 2; x++) vp[x].load(kv, block(next, x), s.h, lane);
+            }
         }
+        s.join(sh, slot, share, a.rw, a.pw, lane);
+        if (s.on && share == 0) s.finish(a, t, it, kv.nkv, slot, lane);
     }
-    s.join(sh, slot, share, a.rw, a.pw, lane);
-    if (s.on && share == 0) s.finish(a, t, it, kv.nkv, slot, lane);
 }
 
 // The same for sequences of several slots over 8-bit caches: the slots' waves
@@ -612,111 +616,115 @@ __global__ __launch_bounds__(512) void k_tree_attn_lds(RowArgs a, KvLayer kv, Tr
     __shared__ __align__(1024) uint8_t ring[NST * STAGE];
     __shared__ int32_t ids[kPartPages];
     Item it;
-    if (!it.read(a, blockIdx.x / kv.nkv)) return;
-    const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int slot = wave % RW, share = wave / RW;
-    const int pages = it.page1 - it.page0, stages = (pages + PPS - 1) / PPS;
-    for (int i = threadIdx.x; i < pages; i += 64 * W) ids[i] = a.btab[it.btab + it.page0 + i];
-    Slot<HD, FMT, QT> s;
-    s.place(t, it, kv.nkv, blockIdx.x % kv.nkv, slot);
-    __syncthreads();
-    // the wave's copies of a stage: codes copy i of page `page`, from byte `off` of its record to byte `to` of the
-    // stage; more copies than there are repeat the last
-    uint32_t off[COPIES];
-    int page[COPIES], to[COPIES];
+    for (int item = blockIdx.x / kv.nkv; item >= 0; item = it.next) {
+        if (!it.read(a, item)) return;
+        int lane = threadIdx.x & 63;
+        asm volatile("" : "+v"(lane));  // as above
+        const int r = lane & 15, g = lane >> 4;
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        const int slot = wave % RW, share = wave / RW;
+        const int pages = it.page1 - it.page0, stages = (pages + PPS - 1) / PPS;
+        for (int i = threadIdx.x; i < pages; i += 64 * W) ids[i] = a.btab[it.btab + it.page0 + i];
+        Slot<HD, FMT, QT> s;
+        s.place(t, it, kv.nkv, blockIdx.x % kv.nkv, slot);
+        __syncthreads();
+        // the wave's copies of a stage: codes copy i of page `page`, from byte `off` of its record to byte `to` of the
+        // stage; more copies than there are repeat the last
+        uint32_t off[COPIES];
+        int page[COPIES], to[COPIES];
 #pragma unroll
-    for (int i = 0; i < COPIES; i++) {
-        const int q = min(wave + W * i, PPS * 2 * CPR - 1), part = q % (2 * CPR), c = (part % CPR * 64 + lane) / 16;
-        page[i] = q / (2 * CPR);
-        to[i] = page[i] * REC + part * 1024;
-        off[i] = part < CPR ? r * HD + c * 16 : 16 * HD + c / CPR * (4 * HD) + r * (HD / 4) + c % CPR * 16;
-    }
-    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)ring;
-    int held = 0, first = -64;  // a lane's block id, of 64 pages from `first` on
-    auto copy = [&](int stage) {
-        const uint32_t at = lds0 + stage % NST * STAGE;
-        const int p0 = stage * PPS;
-        if (p0 >= first + 64) {
-            first = p0;
-            held = ids[min(p0 + lane, pages - 1)];  // past the last page the last again
+        for (int i = 0; i < COPIES; i++) {
+            const int q = min(wave + W * i, PPS * 2 * CPR - 1), part = q % (2 * CPR), c = (part % CPR * 64 + lane) / 16;
+            page[i] = q / (2 * CPR);
+            to[i] = page[i] * REC + part * 1024;
+            off[i] = part < CPR ? r * HD + c * 16 : 16 * HD + c / CPR * (4 * HD) + r * (HD / 4) + c % CPR * 16;
         }
-        auto record = [&](int pg) {
-            const uint32_t id = (uint32_t)__builtin_amdgcn_readlane(held, p0 - first + pg);
-            return kv.data + ((size_t)id * kv.nkv + s.h) * REC;
+        const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)ring;
+        int held = 0, first = -64;  // a lane's block id, of 64 pages from `first` on
+        auto copy = [&](int stage) {
+            const uint32_t at = lds0 + stage % NST * STAGE;
+            const int p0 = stage * PPS;
+            if (p0 >= first + 64) {
+                first = p0;
+                held = ids[min(p0 + lane, pages - 1)];  // past the last page the last again
+            }
+            auto record = [&](int pg) {
+                const uint32_t id = (uint32_t)__builtin_amdgcn_readlane(held, p0 - first + pg);
+                return kv.data + ((size_t)id * kv.nkv + s.h) * REC;
+            };
+#pragma unroll
+            for (int i = 0; i < COPIES; i++) copy_to_lds(at + to[i], record(page[i]), off[i]);
+#pragma unroll
+            for (int i = 0; i < SCOPIES; i++) {
+                const int pg = (wave + W * i) % PPS;
+                if (lane < 8) copy_to_lds(at + pg * REC + 32 * HD, record(pg) + 32 * HD, 16 * lane);
+            }
         };
+        // a pair's record in the ring: pair u of the share's
+        auto pair = [&](int u) { return ring + u / SP % NST * STAGE + ((u % SP * PW + share) * 2) * REC; };
+        auto keys = [&](int u, KeyPage<HD, FMT> (&k)[2]) {
 #pragma unroll
-        for (int i = 0; i < COPIES; i++) copy_to_lds(at + to[i], record(page[i]), off[i]);
+            for (int x = 0; x < 2; x++) {
+                const uint8_t* base = pair(u) + x * REC;
 #pragma unroll
-        for (int i = 0; i < SCOPIES; i++) {
-            const int pg = (wave + W * i) % PPS;
-            if (lane < 8) copy_to_lds(at + pg * REC + 32 * HD, record(pg) + 32 * HD, 16 * lane);
-        }
-    };
-    // a pair's record in the ring: pair u of the share's
-    auto pair = [&](int u) { return ring + u / SP % NST * STAGE + ((u % SP * PW + share) * 2) * REC; };
-    auto keys = [&](int u, KeyPage<HD, FMT> (&k)[2]) {
+                for (int j = 0; j < CPR; j++) {
+                    const u32x4 y = *(const u32x4*)(base + ((g * CPR + j) * 16 + r) * 16);
 #pragma unroll
-        for (int x = 0; x < 2; x++) {
-            const uint8_t* base = pair(u) + x * REC;
-#pragma unroll
-            for (int j = 0; j < CPR; j++) {
-                const u32x4 y = *(const u32x4*)(base + ((g * CPR + j) * 16 + r) * 16);
-#pragma unroll
-                for (int e = 0; e < 4; e++) k[x].d[4 * j + e] = y[e];
+                    for (int e = 0; e < 4; e++) k[x].d[4 * j + e] = y[e];
+                }
+                k[x].s = *(const float4*)(base + 32 * HD + 16 * g);
             }
-            k[x].s = *(const float4*)(base + 32 * HD + 16 * g);
-        }
-    };
-    auto values = [&](int u, ValuePage<HD, FMT> (&v)[2], float (&sc)[8]) {
+        };
+        auto values = [&](int u, ValuePage<HD, FMT> (&v)[2], float (&sc)[8]) {
 #pragma unroll
-        for (int x = 0; x < 2; x++) {
-            const uint8_t* base = pair(u) + x * REC;
-            const float4 z = *(const float4*)(base + 32 * HD + 64 + 16 * g);
-            sc[4 * x] = z.x, sc[4 * x + 1] = z.y, sc[4 * x + 2] = z.z, sc[4 * x + 3] = z.w;
+            for (int x = 0; x < 2; x++) {
+                const uint8_t* base = pair(u) + x * REC;
+                const float4 z = *(const float4*)(base + 32 * HD + 64 + 16 * g);
+                sc[4 * x] = z.x, sc[4 * x + 1] = z.y, sc[4 * x + 2] = z.z, sc[4 * x + 3] = z.w;
 #pragma unroll
-            for (int j = 0; j < CPR; j++) {
-                const u32x4 y = *(const u32x4*)(base + 16 * HD + ((g * CPR + j) * 16 + r) * 16);
+                for (int j = 0; j < CPR; j++) {
+                    const u32x4 y = *(const u32x4*)(base + 16 * HD + ((g * CPR + j) * 16 + r) * 16);
 #pragma unroll
-                for (int e = 0; e < 4; e++) v[x].d[4 * j + e] = y[e];
+                    for (int e = 0; e < 4; e++) v[x].d[4 * j + e] = y[e];
+                }
             }
-        }
-    };
-    for (int i = 0; i < NST - 1; i++) copy(i);
-    s.queries(a, t, it, lane);
-    // This wave's copies of all stages but the last `left` have landed, then everyone's.
+        };
+        for (int i = 0; i < NST - 1; i++) copy(i);
+        s.queries(a, t, it, lane);
+        // This wave's copies of all stages but the last `left` have landed, then everyone's.
 #define LANDED(left)                                                                               \
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((left) * (COPIES + SCOPIES)) : "memory");              \
-    __builtin_amdgcn_s_barrier();                                                                  \
-    asm volatile("" ::: "memory")
-    KeyPage<HD, FMT> kp[2];
-    LANDED(NST - 2);
-    keys(0, kp);
-    for (int st = 0; st < stages; st++) {
-        // the next stage is there too, for the keys that are read ahead, and everyone is past the stage before
-        LANDED(NST - 3);
-        const float none[8] = {};
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"((left) * (COPIES + SCOPIES)) : "memory");              \
+        __builtin_amdgcn_s_barrier();                                                                  \
+        asm volatile("" ::: "memory")
+        KeyPage<HD, FMT> kp[2];
+        LANDED(NST - 2);
+        keys(0, kp);
+        for (int st = 0; st < stages; st++) {
+            // the next stage is there too, for the keys that are read ahead, and everyone is past the stage before
+            LANDED(NST - 3);
+            const float none[8] = {};
 #pragma unroll
-        for (int i = 0; i < SP; i++) {
-            const int u = st * SP + i, p0 = it.page0 + st * PPS + 2 * (i * PW + share);
-            const bool mine = s.on && p0 < s.last;
-            float raw[QT][8], vsc[8];
-            ValuePage<HD, FMT> vp[2];
-            f16x8 hi[QT], lo[QT];
-            if (mine) s.scores(kp, raw, lane);
-            if (i == 0) copy(st + NST - 1);  // over the stage before, its scalar work behind the products
-            if (!mine) continue;
-            values(u, vp, vsc);  // on their way behind the weights
-            s.weights(a, it, p0, raw, vsc, hi, lo, lane);
-            keys(u + 1, kp);  // behind the values' products
-            s.gather(hi, lo, vp, none);
+            for (int i = 0; i < SP; i++) {
+                const int u = st * SP + i, p0 = it.page0 + st * PPS + 2 * (i * PW + share);
+                const bool mine = s.on && p0 < s.last;
+                float raw[QT][8], vsc[8];
+                ValuePage<HD, FMT> vp[2];
+                f16x8 hi[QT], lo[QT];
+                if (mine) s.scores(kp, raw, lane);
+                if (i == 0) copy(st + NST - 1);  // over the stage before, its scalar work behind the products
+                if (!mine) continue;
+                values(u, vp, vsc);  // on their way behind the weights
+                s.weights(a, it, p0, raw, vsc, hi, lo, lane);
+                keys(u + 1, kp);  // behind the values' products
+                s.gather(hi, lo, vp, none);
+            }
         }
-    }
 #undef LANDED
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no copy is left on its way when the ring is reused, or given up
-    __syncthreads();
-    s.join((float*)ring, slot, share, RW, PW, lane);
-    if (s.on && share == 0) s.finish(a, t, it, kv.nkv, slot, lane);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no copy is left on its way when the ring is reused, or given up
+        __syncthreads();
+        s.join((float*)ring, slot, share, RW, PW, lane);
+        if (s.on && share == 0) s.finish(a, t, it, kv.nkv, slot, lane);
+    }
 }
 
 // The parts of each (row, query head), 4 channels a thread. Up to kFewParts: all of them asked for at once, 256
