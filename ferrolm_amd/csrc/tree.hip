@@ -527,8 +527,12 @@ struct Slot {
 }  // namespace
 
 // One workgroup per (kv head, first item of a list): rw row slots x pw position
-// shares, a wave each, which takes its pages from memory straight to registers; the shares'
-// sums meet in LDS.
+// shares, a wave each, which takes its pages from memory straight to registers;
+// the shares' sums meet in LDS. For one slot of rows, where no page is wanted
+// twice, for f32 caches, and for heads of 16 and 32 channels. One token over
+// 1030 cached int8 ones, 32 heads of 64: 7 us, nearly all of it latency (the
+// item, its block ids, pages, the join, one after the other); a tree of 21 rows
+// over as much in f32 14 us.
 template <int HD, int FMT, int QT>
 __global__ __launch_bounds__(512) void k_tree_attn(RowArgs a, KvLayer kv, TreeAttn t) {
     extern __shared__ float sh[];
@@ -599,10 +603,17 @@ __global__ __launch_bounds__(512) void k_tree_attn(RowArgs a, KvLayer kv, TreeAt
 
 // The same for sequences of several slots over 8-bit caches: the slots' waves
 // take each page once, through LDS. A ring of stages (a pair of pages for every
-// position share) is filled by copies from memory straight to LDS, NST - 1 stages ahead, so
+// position share) is filled by copies from memory straight to LDS, three stages ahead, so
 // that enough bytes are on their way to cover the latency of memory: with every
-// wave loading for itself a CU asks for the same 17 KB four times. 16-byte
-// chunks lie in LDS by (chunk, row) so that 16 lanes read 256 consecutive bytes.
+// wave loading for itself a CU asks for the same 17 KB four times (270 us for
+// the case below). 16-byte chunks lie in LDS by (chunk, row) so that 16 lanes
+// read 256 consecutive bytes: no bank conflicts counted.
+// A tree of 29 rows over 131069 fp8 tokens, 8 heads of 128 shared by four: 151
+// us with the merge, 413 TFLOP/s, twice that in matrix work as each product takes
+// two halves. Matrix instructions take 39% of the cycles and vector ones 49%, and
+// with two waves on a SIMD they add up: without the scores the same takes 105
+// us, without the values' product 121, without the weights 121, without the
+// copies 127. Counters in LDS in place of the barriers took 158 against 148.
 template <int HD, int FMT, int RW>
 __global__ __launch_bounds__(512) void k_tree_attn_lds(RowArgs a, KvLayer kv, TreeAttn t) {
     constexpr int QT = 2, PW = RW == 2 ? 4 : 2, W = RW * PW, CPR = HD / 64;  // CPR: 16-byte chunks a lane takes of a page
@@ -728,7 +739,7 @@ __global__ __launch_bounds__(512) void k_tree_attn_lds(RowArgs a, KvLayer kv, Tr
 }
 
 // The parts of each (row, query head), 4 channels a thread. Up to kFewParts: all of them asked for at once, 256
-// threads for as many pairs as they hold.
+// threads for as many pairs as they hold. 3 us for a row, 6 us for 352 rows of 32 heads.
 constexpr int kFewParts = 8;
 template <int HD>
 __global__ __launch_bounds__(256) void k_tree_merge_few(RowArgs a, TreeAttn t, int nkv) {
@@ -770,7 +781,7 @@ __global__ __launch_bounds__(256) void k_tree_merge_few(RowArgs a, TreeAttn t, i
     *(float4*)(t.out + (size_t)row * t.ldo + (size_t)hq * HD + 4 * d) = y;
 }
 
-// More: one workgroup per pair, the parts dealt over its threads.
+// More: one workgroup per pair, the parts dealt over its threads. Tens of parts of 29 rows x 32 heads: 7 us.
 template <int HD>
 __global__ __launch_bounds__(256) void k_tree_merge(RowArgs a, TreeAttn t, int nkv) {
     constexpr int T = HD / 4, NP = 256 / T, QM = HD >= 64 ? 32 : 64;
