@@ -2682,6 +2682,7 @@ int fg_tree_verify(fg_ctx* ctx, const fg_rows* r, int32_t drafts, int32_t vocab,
     int rc;
     if ((rc = check_tree(ctx, r, ld))) return rc;
     if (drafts < FG_DRAFT_EACH || drafts > FG_DRAFT_FIXED || vocab <= 0) return fail(FG_E_ARG, "bad argument");
+    if (vocab > (1 << 30)) return fail(FG_E_SHAPE, "a vocabulary has at most 2^30 tokens");
     if (r->plan.rows == 0) return 0;
     if (!tokens_dev || !p_dev || !u_dev || !out_tokens_dev || !out_path_dev || !out_count_dev ||
         (drafts == FG_DRAFT_FIXED) != !q_dev)

@@ -708,6 +708,8 @@ class Rows:
         self._count(len(seqs))
 
     def set(self, seqs: list) -> None:
+        if not self.ctx.h:
+            raise ValueError("the rows' context is closed")
         arr, keep = _tree_seqs(seqs)
         check(lib().fg_rows_set(self.h, arr, len(seqs)))
         self._count(len(seqs))

@@ -367,9 +367,10 @@ int fg_matmul_device_noalloc(fg_ctx* ctx, const fg_mat* w, const float* x_dev,
 /* Plans rows of `n_seqs` sequences over caches of `kv`'s heads, head_dim and
  * blocks, for `heads` query heads, to be used for every layer of a step; kv
  * NULL plans only their trees (fg_tree_verify, fg_tree_accept; blocks are not
- * read). The host arrays are copied. The handle is the context's, and holds
- * the attention's workspace: its calls run in order on the context's stream,
- * and graphs that captured them share it, so they must not overlap. */
+ * read). The host arrays are copied. The handle is the context's (once that is
+ * destroyed it may only be destroyed itself), and holds the attention's
+ * workspace: its calls run in order on the context's stream, and graphs that
+ * captured them share it, so they must not overlap. */
 int fg_rows_create(fg_ctx* ctx, const fg_kv* kv, int32_t heads,
                    const fg_tree_seq* seqs, int32_t n_seqs, fg_rows** out);
 /* Plans other rows in the same handle (the next step's); calls queued before
@@ -434,7 +435,8 @@ int fg_tree_attention(fg_ctx* ctx, const fg_rows* rows, const fg_kv* kv,
  * out_tokens[s * ld + j], j < out_count[s]: the accepted tokens, then the
  * drawn one; out_path[s * ld + j]: the rows whose distributions they came
  * from, 0 first, so row out_path[j] holds emitted token j - 1. Past the count
- * they hold 0 and -1. ld >= the rows of the longest branch. */
+ * they hold 0 and -1. ld >= the rows of the longest branch. At most 2^30
+ * tokens of a vocabulary. */
 int fg_tree_verify(fg_ctx* ctx, const fg_rows* rows, int32_t drafts,
                    int32_t vocab, const uint32_t* tokens_dev,
                    const float* p_dev, const float* q_dev, const float* u_dev,

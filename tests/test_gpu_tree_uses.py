@@ -286,6 +286,8 @@ def test_refusals_leave_everything_as_it_was(ctx):
             (lambda: gpu.check(gpu.lib().fg_tree_attention(ctx.h, rows.h, c.kv.h, 0, None, 256, out.data_ptr(), 256)),
              "null array"),
             (lambda: gpu.tree_verify(ctx, rows, tok, p, None, u, "each", *res), "come with q"),
+            (lambda: gpu.check(gpu.lib().fg_tree_verify(ctx.h, rows.h, 2, (1 << 30) + 4, tok.data_ptr(), p.data_ptr(), None,
+                                                        u.data_ptr(), *(r.data_ptr() for r in res), rows.deepest)), "2.30 tokens"),
             (lambda: gpu.tree_verify(ctx, rows, tok, p, p, u, "fixed", *res), "come with q"),
             (lambda: gpu.tree_verify(ctx, rows, tok, p, None, u, "fixed", *outputs(1, rows.deepest - 1)), "longest branch"),
             (lambda: gpu.tree_accept(ctx, gpu.Rows(ctx, None, [T(0, None, [-1, -1])]), tok[:2], tok[:2], *outputs(1, 3)),
@@ -317,6 +319,19 @@ def test_refusals_leave_everything_as_it_was(ctx):
     assert rows.total == n  # q = 0: the mean of the values that a row sees
     assert np.abs(out.cpu().numpy() - want.repeat(2, 1)).max() <= bound(0, 0, 30, 1) * np.abs(c.v[0]).max()
     other.close()
+
+
+def test_rows_outlive_their_context_to_be_closed_only():
+    x = gpu.Context(0)
+    kv = gpu.KvCache(x, gpu.CacheShape(1, 1, 64), 4, format="int8")
+    rows = gpu.Rows(x, kv, [gpu.TreeSeq(0, [1], 2)])
+    k = torch.zeros(2, 1, 64, device="cuda")
+    x.close()
+    with pytest.raises(ValueError, match="closed"):
+        rows.set([gpu.TreeSeq(0, [1], 1)])
+    with pytest.raises(gpu.FgError, match="null"):
+        gpu.kv_append(x, rows, kv, 0, k, k)
+    rows.close()
 
 
 def test_nothing_to_do(ctx):
