@@ -40,8 +40,9 @@ constexpr float kLowest = -3e38f;
 // the score would be a whole step of the reference's rounding, and the largest score is to stay its reference.
 constexpr float kFused = 0x1p20f;
 // A weight past kMost, or a probability past kMostP (its value may be zero), raises the reference to where the
-// largest weight is 2^kTop and no probability above 2^kTopP.
-constexpr float kMost = 32768.0f, kMostP = 0x1p60f, kTop = 9.0f, kTopP = 40.0f;
+// largest weight is 2^kTop and no probability above 2^kTopP: weights keep their bits for value scales down to
+// 2^(kTop - kTopP), and 2^30 probabilities have a sum.
+constexpr float kMost = 32768.0f, kMostP = 0x1p90f, kTop = 9.0f, kTopP = 80.0f;
 
 // Eight codes, of which d0 holds the first four, in f16.
 template <int FMT>
@@ -228,7 +229,7 @@ __device__ __forceinline__ void value_scales(const ValuePage<HD, FMT>& p, float*
             for (int i = 0; i < HD / 16; i++) m = fmaxf(m, fabsf(p.d[t][i]) <= 3.4e38f ? fabsf(p.d[t][i]) : INFINITY);
             m = group_reduce<16, true>(m);
             const int e = split_exp(m);
-            s[t] = m < INFINITY ? ldexpf(1.0f, e) : NAN;
+            s[t] = m == 0.0f ? 0.0f : m < INFINITY ? ldexpf(1.0f, e) : NAN;  // zeros leave the reference to others
             f[t] = m < INFINITY ? ldexpf(1.0f, -e) : 0.0f;
         }
     } else {

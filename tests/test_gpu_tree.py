@@ -12,7 +12,13 @@ f16) and 2.5 for f32 keys. A probability is then off by 2 d (its own and its
 sum's), by the exponential (2^-22) and the rounding of its argument (2 eps of
 the largest score, in log 2 units); the weight by its split (2^-21, and f32
 values by theirs, 1.5 x 2^-21); the sums over n tokens by at most n / 4 + 64
-dependent additions. The output is off by sum p |v| times the sum of these."""
+dependent additions. The output is off by sum p |v| times the sum of these.
+That is relative to each weight. A weight (p times its value's scale s, against
+codes up to c) is held to 2^-25 where that is more, half of f16's smallest
+step, while the largest of its sum is 2^9 at least: n such errors times c are
+n c 2^-34 of the largest p s, and c s is the largest |v| of its row: 2^-34 n
+max(p max|v|) more, which shows where the token that has nearly all weight has
+a zero in a channel."""
 import numpy as np
 import pytest
 import torch
@@ -113,6 +119,7 @@ def attention64(q, k, v, visible, fmt):
             out[r, h] = w @ vh[m]
             spread = (np.abs(kh[m]) @ np.abs(q[r, h])).max() / np.sqrt(hd)
             tol[r, h] = w @ np.abs(vh[m]) * bound(spread, np.abs(s).max(), m.sum(), c)
+            tol[r, h] += 2.0 ** -34 * m.sum() * (w * np.abs(vh[m]).max(axis=1)).max()
     return out, tol
 
 

@@ -9,7 +9,7 @@ import pytest
 import torch
 
 from ferrolm_amd import gpu
-from test_gpu_tree import TREES, Case, attention64, bound, cuda, held, sees
+from test_gpu_tree import TREES, Case, attention64, bound, check_attention, cuda, held, sees
 from test_gpu_tree_verify import distributions, drafted, walk
 
 pytestmark = pytest.mark.gpu
@@ -382,3 +382,54 @@ def test_scores_of_any_size(ctx, fmt, sign):
             err = np.abs(out[at + i].cpu().numpy() - v[m].mean(0).repeat(2, 0))
             assert (err <= bound(0, 0, m.sum(), 2.5) * np.abs(v[m]).mean(0).repeat(2, 0)).all()
         at += len(p)
+
+
+@pytest.mark.parametrize("fmt,heads,kv_heads,hd,tree", [
+    ("int8", 16, 8, 128, "deep"), ("fp8", 8, 8, 64, "fan"), ("int8", 8, 8, 128, "one"), ("f32", 32, 8, 32, "forest"),
+    ("fp8", 256, 8, 128, "deep"), ("f32", 16, 8, 64, "one")])
+@pytest.mark.parametrize("seqs", [12, 40, 70])
+def test_batches_around_what_the_card_holds(ctx, fmt, heads, kv_heads, hd, tree, seqs):
+    """Contexts in pieces of their own, in pieces that share a workgroup with others', and whole: fewer sequences
+    than there are places for a kv head (32), somewhat more, and many more, some of them without rows."""
+    rng = np.random.default_rng(seqs)
+    lens = np.exp(rng.uniform(0, np.log(700), seqs)).astype(int)
+    c = Case(ctx, fmt, kv_heads, hd, [(int(n), [] if i % 11 == 5 else TREES[tree]) for i, n in enumerate(lens)], seed=seqs)
+    c.fill()
+    check_attention(c, heads)
+
+
+@pytest.mark.parametrize("fmt,hd,rows", [("int8", 64, 40), ("f32", 16, 1)])
+def test_pieces_end_at_their_most_pages(ctx, fmt, hd, rows):
+    """A context of more pages than a piece holds for each of the two workgroups of a kv head: a workgroup's next
+    piece goes on in it. Its blocks repeat; three of 128 heads are compared."""
+    kv_heads, distinct, pages = 128, 48, 2300
+    c = Case(ctx, fmt, kv_heads, hd, [(distinct * 16, rows)], seed=12)
+    c.fill()
+    first = c.tables[0][:distinct]
+    table = np.concatenate([np.resize(first, pages), c.tables[0][distinct:]])
+    seen = gpu.Rows(ctx, c.kv, [gpu.TreeSeq(pages * 16, table, rows)], heads=kv_heads)
+    q = c.rng.standard_normal((rows, kv_heads, hd)).astype(np.float32)
+    qd, out = cuda(q), torch.empty(rows, kv_heads, hd, device="cuda")
+    torch.cuda.synchronize()
+    gpu.tree_attention(ctx, seen, c.kv, 0, qd, out)
+    ctx.sync()
+    got, some = out.cpu().numpy(), [0, 77, 127]
+    at = np.concatenate([np.resize(np.arange(distinct * 16), pages * 16), distinct * 16 + np.arange(rows)])
+    k, v = (held(x[0][:, some], fmt)[at] for x in (c.k, c.v))
+    pick = [0, rows - 1]
+    want, tol = attention64(q[pick][:, some], k, v, sees(pages * 16, list(range(-1, rows - 1)))[pick], fmt)
+    assert (np.abs(got[pick][:, some] - want) <= tol).all()
+
+
+@pytest.mark.parametrize("fmt", gpu.KV_FORMATS)
+@pytest.mark.parametrize("size", [1e-18, 1e-6, 1e6])
+def test_values_of_any_size(ctx, fmt, size):
+    """The weights' bits do not depend on the size of the values; a context that begins with zeros, and one whose
+    values grow to it."""
+    c = Case(ctx, fmt, 2, 64, [(900, TREES["deep"]), (70, 1), (300, 4)], seed=13)
+    for v in c.v:
+        v *= np.float32(size)
+    c.v[0][:300] = 0
+    c.v[2][:300] *= np.geomspace(1e-3, 1, 300, dtype=np.float32)[:, None, None]
+    c.fill()
+    check_attention(c, 8)
