@@ -98,9 +98,10 @@ __device__ __forceinline__ void split8(const float (&x)[8], f16x8& hi, f16x8& lo
 }
 
 // The exponent that brings values up to m below 2^6 (the two halves then hold them to 2^-31 of m, their products
-// far from f32's ends); bounded, so that 2^-e stays finite.
+// far from f32's ends); bounded, so that 2^-e stays finite. The lowest for zeros, so that values of 0 leave the
+// weights' reference to others.
 __device__ __forceinline__ int split_exp(float m) {
-    int e = 0;
+    int e = -100;
     if (m > 0.0f && m < INFINITY) frexpf(m, &e);
     return max(e, -100) - 6;
 }
@@ -229,7 +230,7 @@ __device__ __forceinline__ void value_scales(const ValuePage<HD, FMT>& p, float*
             for (int i = 0; i < HD / 16; i++) m = fmaxf(m, fabsf(p.d[t][i]) <= 3.4e38f ? fabsf(p.d[t][i]) : INFINITY);
             m = group_reduce<16, true>(m);
             const int e = split_exp(m);
-            s[t] = m == 0.0f ? 0.0f : m < INFINITY ? ldexpf(1.0f, e) : NAN;  // zeros leave the reference to others
+            s[t] = m < INFINITY ? ldexpf(1.0f, e) : NAN;
             f[t] = m < INFINITY ? ldexpf(1.0f, -e) : 0.0f;
         }
     } else {
